@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(HERE, "libdxhip.so")
 
 # Precision bit values, executor/deepxcore/src/deepx/dtype.hpp:120-146
 F64, F32, F16, BF16 = 1 << 0, 1 << 1, 1 << 2, 1 << 3
+F8E4M3 = 1 << 5  # codes of a KvCache only
 I64, I32, I16, I8, BOOL = 1 << 8, 1 << 9, 1 << 10, 1 << 11, 1 << 13
 
 DTYPE_NAMES = {
@@ -64,6 +65,23 @@ class PoolStats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("hits", "misses", "kept", "released", "kept_bytes", "kept_blocks", "live_bytes", "live_blocks")]
 
 
+class Heads(C.Structure):
+    """dxh_heads: a [rows, heads, dim] view, strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Rotary(C.Structure):
+    """dxh_rotary: cosine / sine tables and the rows' positions."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_void_p), ("table_rows", C.c_int64), ("dim", C.c_int32),
+                ("interleaved", C.c_int32), ("position_dtype", C.c_int32)]
+
+
+class NormropePart(C.Structure):
+    """dxh_normrope_part: one tensor of a dxh_normrope / dxh_normrope_backward call."""
+    _fields_ = [("x", Heads), ("y", Heads), ("dx", Heads), ("weight", C.c_void_p), ("dweight", C.c_void_p), ("heads", C.c_int32), ("norm", C.c_int32),
+                ("weight_dtype", C.c_int32)]
+
+
 _p, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _pi32 = C.POINTER(C.c_int32)
 _pp = C.POINTER(C.c_void_p)
@@ -72,6 +90,7 @@ _BIN = [_i, _p, _p, _p, _i64, _p]
 _SCL = [_i, _p, Scalar, _p, _i64, _p]
 _RSCL = [_i, Scalar, _p, _p, _i64, _p]
 _UN = [_i, _p, _p, _i64, _p]
+_i32 = C.c_int32
 _RED = [_i, _p, _pi32, _i, _pi32, _i, _p, _p, _sz, _p]
 
 ABI_VERSION = 200  # DXH_ABI_VERSION of include/dxhip.h, the layout SIGNATURES below describes
@@ -150,6 +169,9 @@ SIGNATURES = {
     "dxh_matmul": ([_i, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _sz, _p], _i),
     "dxh_matmul_shared_a_workspace_bytes": ([_i, _p, _pp, _pp, _i, _i64, _i64, _i64, C.POINTER(_sz)], _i),
     "dxh_matmul_shared_a": ([_i, _p, _pp, _pp, _i, _i64, _i64, _i64, _p, _sz, _p], _i),
+    "dxh_normrope": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, _f, C.POINTER(Rotary), _p], _i),
+    "dxh_normrope_backward_workspace_bytes": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, C.POINTER(_sz)], _i),
+    "dxh_normrope_backward": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, _f, C.POINTER(Rotary), _p, _sz, _p], _i),
 }
 
 _lib = None

@@ -53,6 +53,7 @@ enum dxh_dtype {
     DXH_F32  = 1 << 1,
     DXH_F16  = 1 << 2,
     DXH_BF16 = 1 << 3,
+    DXH_F8E4M3 = 1 << 5, /* float8 e4m3 without infinities (largest value 448): codes of a dxh_kvcache only */
     DXH_I64  = 1 << 8,
     DXH_I32  = 1 << 9,
     DXH_I16  = 1 << 10,
@@ -470,6 +471,58 @@ DXH_API int dxh_matmul_shared_a_workspace_bytes(int dtype, const void *a, const 
                                                 int64_t m, int64_t k, int64_t n, size_t *bytes);
 DXH_API int dxh_matmul_shared_a(int dtype, const void *a, const void *const *bs, void *const *cs, int count, int64_t m,
                                 int64_t k, int64_t n, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- attention: the steps between the q / k / v products and the output product of a decoder layer
+ * No counterpart in the reference's executors, whose front spells them as separate instructions: the rotation as
+ * sin / cos / mul / add / concat (front/py/deepx/nn/modules/transformer/rotary_embedding.py:50-71), the attention as
+ * matmul + softmax + matmul over tensors that it keeps whole
+ * (front/py/deepx/nn/modules/transformer/attention.py:15-32).
+ *
+ * dxh_heads is a [rows, heads, dim] view: element (r, h, d) at data[r * row_stride + h * head_stride + d], strides in
+ * elements.  `dim` values of a head are contiguous; data and both strides are multiples of 16 bytes, else
+ * DXH_ERR_ALIGN.  The query heads of a row of a q | k | v product are such a view, and so are the heads of a
+ * [heads, rows, dim] tensor. */
+typedef struct dxh_heads {
+    void *data;
+    int64_t row_stride, head_stride;
+} dxh_heads;
+
+/* RMS norm of every head and its position rotation in one pass, for up to DXH_NORMROPE_MAX_PARTS tensors (the queries and
+ * the keys of the same rows) in one launch.
+ *   n = x * weight / sqrt(mean(x^2) + eps) over the head's `dim` values (norm = 0: n = x; weight NULL: all ones);
+ *   of the first rotary.dim values the pairs (i, i + rotary.dim/2), or (2i, 2i + 1) with `interleaved`, are turned by the
+ *   angle whose cosine and sine are cos[p][i] and sin[p][i], p = positions[row]:  y_a = n_a c - n_b s,  y_b = n_b c + n_a s;
+ *   the other values of the head pass unchanged.
+ * Computed in fp32, one rounding of the result.  cos / sin: fp32 [table_rows, rotary.dim / 2]; a position outside the table
+ * is clamped into it; positions NULL: 0, 1, 2 ...  rotary NULL or rotary.dim = 0: no rotation.  y may be x itself (the same
+ * pointer and strides); any other overlap is not allowed.  dtypes f32 f16 bf16, weights of the same dtype or f32, dim a
+ * multiple of 16 up to 256, rotary.dim any even number up to dim. */
+#define DXH_NORMROPE_MAX_PARTS 4
+typedef struct dxh_rotary {
+    const float *cos, *sin;
+    const void *positions;   /* [rows] of position_dtype, or NULL */
+    int64_t table_rows;
+    int32_t dim, interleaved;
+    int32_t position_dtype;  /* DXH_I32 or DXH_I64 */
+} dxh_rotary;
+typedef struct dxh_normrope_part {
+    dxh_heads x;
+    dxh_heads y;          /* forward: the result; backward: the gradient that comes in */
+    dxh_heads dx;         /* backward: the gradient of x (may be y itself); forward: not used */
+    const void *weight;   /* [dim], or NULL */
+    float *dweight;       /* backward: [dim] fp32, overwritten, or NULL; forward: not used */
+    int32_t heads, norm;  /* norm: 1 on, 0 off */
+    int32_t weight_dtype;
+} dxh_normrope_part;
+DXH_API int dxh_normrope(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, int32_t dim, float eps,
+                         const dxh_rotary *rotary, void *stream);
+/* Its gradients, from the same x, weight, tables and positions: dx of every element and, where dweight is given, the
+ * weight's gradient summed over rows and heads in fp32 in a fixed order (the same bits on every run).  `workspace`: device
+ * memory of the caller of at least the query's bytes, 16-byte aligned, that no other call in flight uses; it may be NULL
+ * when the query reports 0 (no dweight). */
+DXH_API int dxh_normrope_backward_workspace_bytes(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, int32_t dim, size_t *bytes);
+DXH_API int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, int32_t dim, float eps,
+                                  const dxh_rotary *rotary, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -82,6 +82,17 @@ class NormropePart(C.Structure):
                 ("weight_dtype", C.c_int32)]
 
 
+class KvCache(C.Structure):
+    """dxh_kvcache: a paged cache of keys and values in 8 bits."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("page_table", C.c_void_p), ("num_pages", C.c_int64),
+                ("pages_per_seq", C.c_int32), ("page_size", C.c_int32), ("heads", C.c_int32), ("dim", C.c_int32), ("code", C.c_int32)]
+
+
+class KvRows(C.Structure):
+    """dxh_kvrows: which packed rows belong to which sequence of a cache."""
+    _fields_ = [("offsets", C.c_void_p), ("lengths", C.c_void_p), ("rows", C.c_int64), ("batch", C.c_int32), ("max_rows", C.c_int32)]
+
+
 _p, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _pi32 = C.POINTER(C.c_int32)
 _pp = C.POINTER(C.c_void_p)
@@ -91,6 +102,7 @@ _SCL = [_i, _p, Scalar, _p, _i64, _p]
 _RSCL = [_i, Scalar, _p, _p, _i64, _p]
 _UN = [_i, _p, _p, _i64, _p]
 _i32 = C.c_int32
+_KV = [C.POINTER(KvCache), C.POINTER(KvRows), _i, C.POINTER(Heads), C.POINTER(Heads), _p]
 _RED = [_i, _p, _pi32, _i, _pi32, _i, _p, _p, _sz, _p]
 
 ABI_VERSION = 200  # DXH_ABI_VERSION of include/dxhip.h, the layout SIGNATURES below describes
@@ -172,6 +184,9 @@ SIGNATURES = {
     "dxh_normrope": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, _f, C.POINTER(Rotary), _p], _i),
     "dxh_normrope_backward_workspace_bytes": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, C.POINTER(_sz)], _i),
     "dxh_normrope_backward": ([_i, C.POINTER(NormropePart), _i, _i64, _i32, _f, C.POINTER(Rotary), _p, _sz, _p], _i),
+    "dxh_kvcache_write": (_KV, _i), "dxh_kvcache_read": (_KV, _i),
+    "dxh_kvcache_attention_workspace_bytes": ([C.POINTER(KvCache), C.POINTER(KvRows), _i, _i32, C.POINTER(_sz)], _i),
+    "dxh_kvcache_attention": ([C.POINTER(KvCache), C.POINTER(KvRows), _i, _i32, C.POINTER(Heads), C.POINTER(Heads), _p, _f, _i, _i64, _p, _sz, _p], _i),
 }
 
 _lib = None

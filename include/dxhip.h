@@ -524,6 +524,67 @@ DXH_API int dxh_normrope_backward_workspace_bytes(int dtype, const dxh_normrope_
 DXH_API int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, int32_t dim, float eps,
                                   const dxh_rotary *rotary, void *workspace, size_t workspace_bytes, void *stream);
 
+/* A cache of keys and values in 8 bits, one fp32 scale for each page (a block of page_size consecutive tokens of one
+ * sequence) and head: value = code * scale.  Device memory of the caller:
+ *   k        [num_pages, heads, page_size, dim]   codes, a page's tokens of one head in a row
+ *   v        [num_pages, heads, dim, page_size]   codes, tokens innermost: the order in which the attention multiplies them
+ *   k_scale, v_scale  [num_pages, heads]
+ *   page_table        [batch, pages_per_seq] int32: the page that holds tokens i * page_size ... of sequence b; NULL: page
+ *                     b * pages_per_seq + i (a cache without paging).  An entry outside [0, num_pages) is no page: nothing
+ *                     is written there, reads give zeros, the attention sees no tokens in it.
+ * code: DXH_I8 or DXH_F8E4M3.  page_size 16, 32, 64 or 128; dim a multiple of 16 up to 256; k and v 16-byte aligned.
+ *
+ * The rows of a call are packed [rows, heads, dim]: sequence b has the rows offsets[b] .. offsets[b + 1] - 1 (device int32
+ * [batch + 1], ascending), and they are the last of the lengths[b] tokens (device int32 [batch]) that the sequence holds in
+ * the cache: row i of its n rows is the token at lengths[b] - n + i.  offsets NULL: every sequence has max_rows rows.
+ * max_rows (host) is the most rows any sequence has.  A row before token 0 or at or past token pages_per_seq * page_size
+ * has no place in the cache: it is not written and reads as zeros.  Rows of a sequence beyond max_rows and rows behind the
+ * last sequence are left as they are; offsets outside [0, rows] are clamped into it: no content of the device arrays makes
+ * a call touch memory outside its tensors.
+ * Nothing of the device arrays is read on the host, so a recorded graph follows them as they change. */
+typedef struct dxh_kvcache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t *page_table;
+    int64_t num_pages;
+    int32_t pages_per_seq, page_size, heads, dim;
+    int32_t code;
+} dxh_kvcache;
+typedef struct dxh_kvrows {
+    const int32_t *offsets, *lengths;
+    int64_t rows;
+    int32_t batch, max_rows;
+} dxh_kvrows;
+
+/* Quantises new keys and values into the cache.  For every page and head that rows fall into, in fp32 with one rounding a step:
+ *   top   = the largest |x| among them (NaN ignored, infinities as FLT_MAX)
+ *   scale = max(top * c, 2^-100), c = the fp32 value nearest to 1/127 (int8) or 1/448 (e4m3); if the page holds older tokens
+ *           of the sequence (before the first row) at least its old scale
+ *   code  = x * (1 / scale), clamped to +-127 or +-448, rounded to nearest even (a NaN becomes 0 in int8, NaN in e4m3)
+ * and, if older tokens are there and the scale grew, their codes become code * (old scale * (1 / scale)) rounded the same way.
+ * Codes of a page behind the last row are left as they are.  The pages that two sequences write must differ (a page shared
+ * as a common prefix may be read by many, but its table entry must not be one that a row falls into). */
+DXH_API int dxh_kvcache_write(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, const dxh_heads *k, const dxh_heads *v, void *stream);
+/* The values of those rows back: code * scale in fp32, rounded once to dtype (f32 f16 bf16). */
+DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, const dxh_heads *k, const dxh_heads *v, void *stream);
+
+/* Attention of the rows over the cache: for a row at position p of its sequence and query head h,
+ *   out = sum_j softmax_j(scale * q . k_j) v_j   over the tokens j < lengths[b] it sees: with `causal` j <= p, with window > 0
+ *   j > p - window; key head h / (q_heads / heads).
+ * A row that sees no token gives zeros (lse: -infinity).  lse, if not NULL: [rows, q_heads] fp32, the natural logarithm of
+ * the sum of exp(scale * q . k_j).  What tokens that a row does not see hold has no effect on it, NaN codes and scales of
+ * pages without visible tokens included; a NaN among a visible token's values makes that dimension of the row, or the whole
+ * row, NaN.  dtype f32 f16 bf16 for q and out (which must not overlap); q_heads a multiple of cache->heads.  Scores,
+ * maxima, sums and the output are accumulated in fp32; a probability is rounded to bf16 for a bf16 row, kept to 16 bits of
+ * precision for f16 and to 24 for f32; codes enter the products exactly.
+ * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a
+ * second launch: device memory of the caller of at least the query's bytes, 256-byte aligned, that no other call in flight
+ * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows and q_heads alone; workspace may be NULL when it is 0. */
+DXH_API int dxh_kvcache_attention_workspace_bytes(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_heads, size_t *bytes);
+DXH_API int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_heads, const dxh_heads *q,
+                                  const dxh_heads *out, float *lse, float scale, int causal, int64_t window, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -64,3 +64,67 @@ def test_normrope_backward():
     assert back(norm_part(), None, 0) == WORKSPACE and back(norm_part(), 4096, 16) == WORKSPACE and back(norm_part(), 4100, 1 << 30) == WORKSPACE
     assert back(norm_part(dx=dx.Heads()), 4096, 1 << 30) == ARG and back(norm_part(dx=heads(4100)), 4096, 1 << 30) == ALIGN and back(norm_part(dweight=513), 4096, 1 << 30) == ALIGN
     assert L.dxh_normrope_backward_workspace_bytes(dx.BF16, (dx.NormropePart * 1)(norm_part(dweight=None)), 1, 100, 64, C.byref(n)) == OK and n.value == 0
+
+
+def cache(**kw):
+    c = dx.KvCache(4096, 8192, 256, 512, 1024, 100, 8, 16, 2, 64, dx.I8)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def kvrows(**kw):
+    r = dx.KvRows(256, 512, 0, 4, 8)
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+BAD_CACHE = [(dict(code=dx.I16), DTYPE), (dict(code=dx.BF16), DTYPE), (dict(num_pages=-1), ARG), (dict(pages_per_seq=-1), ARG), (dict(heads=0), ARG), (dict(page_size=8), SHAPE),
+             (dict(page_size=48), SHAPE), (dict(page_size=256), SHAPE), (dict(dim=24), SHAPE), (dict(dim=272), SHAPE), (dict(dim=0), SHAPE), (dict(k=4100), ALIGN), (dict(v=8193), ALIGN),
+             (dict(k_scale=258), ALIGN), (dict(page_table=1026), ALIGN), (dict(page_table=None, num_pages=31), SHAPE)]
+BAD_ROWS = [(dict(batch=-1), ARG), (dict(rows=-1), ARG), (dict(max_rows=-1), ARG), (dict(offsets=258), ALIGN), (dict(lengths=514), ALIGN), (dict(offsets=None, rows=31), SHAPE),
+            (dict(rows=1 << 31), -6), (dict(rows=1, lengths=None), ARG)]
+
+
+def test_kvcache_write_and_read():
+    L = dx.load()
+    for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
+        call = lambda c=None, r=None, dtype=dx.BF16, k=None, v=None: fn(c or cache(), r or kvrows(), dtype, k or heads(), v or heads(), None)  # noqa: E731, B023
+        assert call() == OK and call(cache(code=dx.F8E4M3)) == OK and call(cache(page_table=None, num_pages=32)) == OK
+        for kw, rc in BAD_CACHE:
+            assert call(cache(**kw)) == rc, kw
+        for kw, rc in BAD_ROWS:
+            assert call(r=kvrows(**kw)) == rc, kw
+        assert call(r=kvrows(rows=1), c=cache(k=None)) == ARG and call(r=kvrows(rows=1), c=cache(v_scale=None)) == ARG
+        assert call(dtype=dx.F64) == DTYPE and call(dtype=dx.I8) == DTYPE
+        assert fn(None, kvrows(), dx.BF16, heads(), heads(), None) == ARG and fn(cache(), None, dx.BF16, heads(), heads(), None) == ARG
+        assert fn(cache(), kvrows(), dx.BF16, None, heads(), None) == ARG
+        assert call(r=kvrows(rows=1), k=dx.Heads()) == ARG and call(k=heads(4100)) == ALIGN and call(v=heads(row=1028)) == ALIGN and call(v=heads(head=60)) == ALIGN
+        assert call(r=kvrows(rows=1 << 30, batch=1 << 20, max_rows=1 << 20)) == -6  # more workgroups than a launch has
+
+
+def test_kvcache_attention():
+    L = dx.load()
+    n = C.c_size_t(1)
+
+    def att(c=None, r=None, dtype=dx.BF16, q_heads=14, q=None, out=None, lse=None, scale=0.125, causal=1, window=0, ws=None, nbytes=0):
+        return L.dxh_kvcache_attention(c or cache(), r or kvrows(), dtype, q_heads, q or heads(), out or heads(8192), lse, scale, causal, window, ws, nbytes, None)
+
+    query = lambda c=None, r=None, dtype=dx.BF16, q_heads=14: L.dxh_kvcache_attention_workspace_bytes(c or cache(), r or kvrows(), dtype, q_heads, C.byref(n))  # noqa: E731
+    assert att() == OK and query() == OK and n.value == 0
+    for kw, rc in BAD_CACHE:
+        assert att(cache(**kw)) == rc and query(cache(**kw)) == rc, kw
+    for kw, rc in BAD_ROWS:
+        assert att(r=kvrows(**kw)) == rc and query(r=kvrows(**kw)) == rc, kw
+    assert att(q_heads=0) == ARG and att(q_heads=15) == SHAPE and query(q_heads=15) == SHAPE and query(q_heads=-2) == ARG and query(dtype=dx.F64) == DTYPE
+    assert L.dxh_kvcache_attention_workspace_bytes(cache(), kvrows(), dx.BF16, 14, None) == ARG
+    assert att(causal=2) == ARG and att(window=-1) == ARG and att(scale=float("nan")) == ARG and att(scale=float("inf")) == ARG
+    assert att(lse=258) == ALIGN and att(q=heads(4098)) == ALIGN and att(out=heads(head=65)) == ALIGN
+    assert att(r=kvrows(rows=1), q=dx.Heads()) == ARG and att(r=kvrows(rows=1), out=dx.Heads()) == ARG
+    assert att(r=kvrows(rows=1 << 30, batch=1, max_rows=1 << 30), q_heads=14) == -6
+    # a long cache under one row is cut: the workspace is asked for and checked
+    long = cache(num_pages=100000, pages_per_seq=8192)
+    one = kvrows(rows=1, batch=1, max_rows=1)
+    assert query(long, one) == OK and n.value > 0
+    assert att(long, one) == WORKSPACE and att(long, one, ws=4096, nbytes=n.value - 1) == WORKSPACE and att(long, one, ws=4096 + 16, nbytes=n.value) == WORKSPACE

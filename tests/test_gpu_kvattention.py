@@ -1,0 +1,233 @@
+"""dxh_kvcache_attention against a 64-bit softmax over the tokens a row sees (tests/kv_reference.py, where the bars are derived)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from deepx_amd import lib as dx
+from tests import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def call(L, cache, rows_desc, name, q, out, lse, scale, causal, window, st=None, ws=None):
+    need = C.c_size_t(0)
+    dx.check(L.dxh_kvcache_attention_workspace_bytes(cache, rows_desc, R.DT[name], q.shape[1], C.byref(need)), "query")
+    if ws is None:
+        ws = torch.empty(max(1, need.value), dtype=torch.uint8, device="cuda")
+    assert ws.numel() >= need.value
+    dx.check(L.dxh_kvcache_attention(cache, rows_desc, R.DT[name], q.shape[1], R.heads(q), R.heads(out), lse.data_ptr() if lse is not None else None, scale, causal, window, ws.data_ptr(),
+                                     need.value, stream() if st is None else st), "attention")
+    return ws
+
+
+def check(L, c, rows, name, q_heads, causal=1, window=0, scale=None, q=None, seed=0, size=1.0):
+    scale = c.dim ** -0.5 if scale is None else scale
+    if q is None:
+        q = torch.randn(rows.rows, q_heads, c.dim, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") * size
+    q = q.to(R.TT[name])
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    ws = call(L, c.upload(), rows.upload(), name, q, out, lse, scale, causal, window)
+    want = R.attention(c, rows, q.double().cpu().numpy(), scale, causal, window)
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert ws is not None
+    for r in range(rows.rows):
+        if r not in want:  # rows behind the last sequence or beyond max_rows
+            assert (got[r] == 7.0).all() and (got_lse[r] == 7.0).all(), r
+            continue
+        bar, lse_bar = R.attention_bar(name, c, want[r])
+        assert np.array_equal(np.isinf(got_lse[r]), np.isinf(want[r][1])), r
+        err = np.abs(got[r] - want[r][0])
+        worst = float((err / bar).max())
+        assert worst <= 1, (r, worst)
+        fine = np.isfinite(want[r][1])
+        assert (np.abs(got_lse[r][fine] - want[r][1][fine]) <= lse_bar[fine]).all(), r
+    return out
+
+
+# code, page, key heads, query heads, dim, counts, lengths
+CASES = [
+    ("i8", 16, 1, 1, 64, (1,), (1,)), ("e4m3", 16, 2, 14, 64, (1, 1, 1), (1, 64, 65)), ("i8", 16, 2, 14, 64, (1,), (777,)), ("e4m3", 32, 1, 16, 128, (1, 1), (63, 500)),
+    ("i8", 64, 1, 17, 128, (1, 1), (129, 1)), ("e4m3", 128, 3, 3, 80, (2, 5, 1), (2, 130, 255)), ("i8", 16, 2, 4, 16, (3, 0, 4), (30, 9, 4)), ("i8", 32, 1, 2, 96, (33, 7), (40, 200)),
+    ("e4m3", 64, 2, 10, 256, (4, 1), (100, 321)), ("i8", 128, 1, 8, 192, (1, 9), (300, 9)), ("e4m3", 16, 1, 5, 48, (70, 1, 17), (70, 90, 100)), ("i8", 64, 4, 4, 32, (130, 65), (130, 150)),
+    ("e4m3", 64, 1, 4, 128, (200,), (231,)), ("i8", 16, 1, 7, 64, (129,), (140,)),
+]
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_ragged(dxh, case, name):
+    code, page, hk, hq, dim, counts, lengths = case
+    c = R.Cache(code, page, hk, dim, len(counts), -(-max(lengths) // page), seed=dim + hq)
+    check(dxh, c, R.Rows(counts, lengths, extra=1), name, hq)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("window", [0, 1, 2, 63, 64, 65, 200, 2 ** 40])
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_masks(dxh, code, window, causal, name):
+    """sliding windows with and without the causal limit over chunks of rows that begin inside and at the edges of tiles"""
+    c = R.Cache(code, 16, 1, 64, 3, 20, seed=window % 97)
+    check(dxh, c, R.Rows((70, 1, 33), (300, 257, 33)), name, 3, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_what_a_row_does_not_see_has_no_effect(dxh, code, name):
+    """missing pages, rows without tokens, lengths of zero, past the table and negative, rows beyond max_rows; every code that no row sees is the
+    worst there is (NaN in e4m3), every scale of a page that no row sees is NaN"""
+    for rows in (R.Rows((5, 3, 40, 2, 1, 9), (90, 1, 20, 0, 16, 200), extra=2, max_rows=30), R.Rows((1, 1, 1, 1, 1, 1), (0, -5, 2 ** 31 - 1, 33, 17, 96))):
+        c = R.Cache(code, 16, 2, 64, 6, 6, seed=3, missing=[(0, 1, -1), (1, 0, 1 << 30), (2, 5, -7), (4, 0, -1)])
+        seen = np.zeros((c.pages, 16), bool)
+        for b, r, t in rows.each():
+            for j in range(0, min(t + 1, rows.lengths[b], 96) if t >= 0 else 0):
+                if c.page_of(b, j // 16) >= 0:
+                    seen[c.page_of(b, j // 16), j % 16] = True
+        c.k[~np.broadcast_to(seen[:, None, :, None], c.k.shape)] = 127  # 0x7f: NaN in e4m3
+        c.v[~np.broadcast_to(seen[:, None, None, :], c.v.shape)] = 127
+        c.ks[~seen.any(1)] = np.nan
+        c.vs[~seen.any(1)] = np.inf
+        check(dxh, c, rows, name, 6)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_nan_of_a_later_token(dxh, name):
+    """a NaN among the values (and, of another token, the keys) of a token: rows before it are as without it, rows that see it are NaN"""
+    for kind in ("k", "v"):
+        c = R.Cache("e4m3", 16, 1, 64, 1, 8, seed=4)
+        rows = R.Rows((100,), (120,))
+        q = torch.randn(100, 3, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+        clean = check(dxh, c, rows, name, 3, q=q)
+        p, token = c.page_of(0, 70 // 16), 70 % 16
+        if kind == "k":
+            c.k[p, 0, token, 5] = 127
+        else:
+            c.v[p, 0, 5, token] = -1
+        out = torch.full_like(clean, 7.0)
+        call(dxh, c.upload(), rows.upload(), name, q.to(R.TT[name]), out, None, 0.125, 1, 0)
+        sees = torch.arange(100) + 20 >= 70
+        assert torch.equal(out[~sees], clean[~sees]) and torch.isnan(out[sees][..., 5]).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_long_sequences_in_slices(dxh, code, name):
+    """few rows over long ragged sequences: the tokens are cut into slices and joined; the same bits twice"""
+    c = R.Cache(code, 64, 1, 64, 3, 80, seed=6)
+    rows = R.Rows((1, 3, 2), (5000, 70, 2049))
+    need = C.c_size_t(0)
+    dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], 4, C.byref(need)))
+    assert need.value > 0
+    a = check(dxh, c, rows, name, 4)
+    b = check(dxh, c, rows, name, 4)
+    assert torch.equal(a, b)
+    check(dxh, c, rows, name, 4, window=700)
+
+
+@pytest.mark.parametrize("size", [0.0, 30.0, 3000.0])
+def test_flat_and_peaked_scores(dxh, size):
+    """all scores equal; scores so large that one token takes everything"""
+    c = R.Cache("i8", 32, 1, 128, 2, 10, seed=8)
+    check(dxh, c, R.Rows((3, 40), (300, 64)), "f32", 2, size=size)
+    check(dxh, c, R.Rows((3, 40), (300, 64)), "bf16", 2, size=size, scale=-0.1)
+
+
+def test_page_scales_of_very_different_size(dxh):
+    c = R.Cache("i8", 16, 1, 64, 1, 40, seed=9)
+    c.vs *= np.float32(10.0) ** np.random.default_rng(1).integers(-20, 20, c.vs.shape).astype(np.float32)
+    for name in ("f32", "bf16"):
+        check(dxh, c, R.Rows((40,), (600,)), name, 2)
+    c.vs[:] = 0  # a cache of zeros
+    check(dxh, c, R.Rows((1,), (600,)), "f32", 2)
+
+
+def test_without_table_or_offsets_strided_and_shared_pages(dxh):
+    c = R.Cache("i8", 16, 2, 64, 3, 5, seed=10, paged=False)
+    check(dxh, c, R.Rows((4,) * 3, (5, 80, 33), uniform=True), "bf16", 4)
+    # a prefix that two sequences share, and the same page twice in one
+    c = R.Cache("e4m3", 16, 2, 64, 2, 5, seed=11)
+    c.table[1, :3] = c.table[0, :3]
+    c.table[0, 4] = c.table[0, 0]
+    check(dxh, c, R.Rows((2, 3), (80, 70)), "f32", 4)
+    # [heads, rows, dim] views in and out, no lse
+    rows = R.Rows((20, 3), (30, 70))
+    q = torch.randn(4, 23, 64, device="cuda").transpose(0, 1)
+    want, out = torch.empty(23, 4, 64, device="cuda"), torch.empty(4, 23, 64, device="cuda").transpose(0, 1)
+    call(dxh, c.upload(), rows.upload(), "f32", q.contiguous(), want, None, 0.125, 1, 0)
+    call(dxh, c.upload(), rows.upload(), "f32", q, out, None, 0.125, 1, 0)
+    assert torch.equal(out, want)
+
+
+def test_recorded_and_replayed_as_sequences_grow(dxh):
+    """one graph of a decode step, replayed while lengths and rows change under it, with eager calls between on another stream's workspace"""
+    c = R.Cache("e4m3", 16, 1, 64, 2, 200, seed=12)
+    rows = R.Rows((1, 1), (100, 2500))
+    cache, desc = c.upload(), rows.upload()
+    q = torch.randn(2, 7, 64, device="cuda").bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(2, 7, device="cuda")
+    st, graph = C.c_void_p(), C.c_void_p()
+    dx.check(dxh.dxh_stream_create(C.byref(st)))
+    need = C.c_size_t(0)
+    dx.check(dxh.dxh_kvcache_attention_workspace_bytes(cache, desc, dx.BF16, 7, C.byref(need)))
+    ws = torch.empty(max(1, need.value), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    dx.check(dxh.dxh_graph_begin_capture(st))
+    call(dxh, cache, desc, "bf16", q, out, lse, 0.125, 1, 0, st=st, ws=ws)
+    dx.check(dxh.dxh_graph_end_capture(st, C.byref(graph)))
+    for step in range(4):
+        rows.dev[1].copy_(torch.tensor([100 + step * 300, 2500 + 64 * step], dtype=torch.int32))
+        q.copy_(torch.randn(2, 7, 64, device="cuda"))
+        eager, eager_lse = torch.empty_like(out), torch.empty_like(lse)
+        call(dxh, cache, desc, "bf16", q, eager, eager_lse, 0.125, 1, 0)
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        dx.check(dxh.dxh_graph_launch(graph, st))
+        dx.check(dxh.dxh_stream_sync(st))
+        assert torch.equal(out, eager) and torch.equal(lse, eager_lse)
+    dx.check(dxh.dxh_graph_destroy(graph))
+    dx.check(dxh.dxh_stream_destroy(st))
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_as_they_are_used_together(dxh, code):
+    """a prompt and then tokens one by one: rotation, cache, attention, each step against the 64-bit attention over what the cache holds, and the
+    attention over the cache against the attention over unquantised keys and values (off by what 8 bits cost: a code is off by half a step of
+    max|x| / 127, or by 2^-4 of a value in e4m3)"""
+    hq, hk, dim, page = 6, 2, 64, 16
+    c = R.Cache(code, page, hk, dim, 2, 8, seed=13)
+    cache = c.upload()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    angle = torch.arange(128, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))
+    cos, sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+    wq, wk = torch.randn(dim, generator=g, device="cuda"), torch.randn(dim, generator=g, device="cuda")
+    have = [0, 0]
+    for counts in ((37, 80), (1, 1), (1, 1), (2, 0)):
+        have = [a + b for a, b in zip(have, counts)]
+        rows = R.Rows(counts, have)
+        desc = rows.upload()
+        pos = torch.tensor([t for _, _, t in rows.each()], dtype=torch.int32, device="cuda")
+        qkv = torch.randn(rows.rows, (hq + 2 * hk) * dim, generator=g, device="cuda")
+        q, k, v = (t.view(rows.rows, -1, dim) for t in qkv.split([hq * dim, hk * dim, hk * dim], 1))
+        part = lambda x, w: dx.NormropePart(R.heads(x), R.heads(x), dx.Heads(), w.data_ptr(), None, x.shape[1], 1, dx.F32)  # noqa: E731
+        rot = dx.Rotary(cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), 128, dim, 0, dx.I32)
+        dx.check(dxh.dxh_normrope(dx.F32, (dx.NormropePart * 2)(part(q, wq), part(k, wk)), 2, rows.rows, dim, 1e-6, rot, stream()))
+        dx.check(dxh.dxh_kvcache_write(cache, desc, dx.F32, R.heads(k), R.heads(v), stream()))
+        out = torch.empty(rows.rows, hq, dim, device="cuda")
+        call(dxh, cache, desc, "f32", q, out, None, dim ** -0.5, 1, 0)
+        c.k, c.v, c.ks, c.vs = c.download()
+        want = R.attention(c, rows, q.double().cpu().numpy(), dim ** -0.5, 1, 0)
+        for r, entry in want.items():
+            assert (np.abs(out[r].double().cpu().numpy() - entry[0]) <= R.attention_bar("f32", c, entry)[0]).all()
+        back = [torch.empty_like(k), torch.empty_like(v)]
+        dx.check(dxh.dxh_kvcache_read(cache, desc, dx.F32, R.heads(back[0]), R.heads(back[1]), stream()))
+        for b, x in zip(back, (k, v)):
+            # the page's scale is from the largest value ever in it: at most that of all rows so far (unit normal rows: below 6 here; keys times their weight)
+            step = 6 * max(1.0, float(wk.abs().max())) * dim ** 0.5 / 127 / 2 if code == "i8" else 0
+            bound = step if code == "i8" else x.abs() * 2 ** -4 + 6 * max(1.0, float(wk.abs().max())) * dim ** 0.5 / 448 * 2 ** -10
+            assert ((b - x).abs() <= bound).all()

@@ -1,19 +1,23 @@
 // kvattention.hip — attention of a ragged batch of rows over a paged cache in 8 bits.
 //
 // For one key head and one sequence the rows of all query heads that share it are one matrix Q [R, D], row r = i * G + g for
-// query row i and head g of the G that share the key head.  With K' = the key codes, one pass over the tokens keeps for every row
-//     s_j = (Q K'^T)_j * k_scale(page of j) * scale * log2(e),     m = max s_j,  l = sum 2^(s_j - m),
-//     O   = sum 2^(s_j - m) v_scale(page of j) V'_j;               out = O / l,  lse = ln 2 (m + log2 l).
-// Codes are whole numbers below 2^8 or e4m3 values: both are exact in bf16, so they enter the matrix pipe exactly and the
-// scales are applied to scores and probabilities in fp32.  A probability (with its v_scale) is rounded to bf16 for bf16 rows
-// (2^-9 of each term, random signs: under the rounding of the result); f16 rows split Q and P into two bf16 parts and f32 rows
-// into three (16 and 24 bits), each part one more product.
+// query row i and head g of the G that share the key head.  With codes K', V' and page scales k_s, v_s, in base 2:
+//     s_j = (Q K'^T)_j k_s(j) scale log2(e),     t_j = s_j + log2 v_s(j),     m = max t_j,     p_j = 2^(t_j - m),
+//     O   = sum p_j V'_j,     l = sum p_j / v_s(j),     out = O / l,     lse = ln 2 (m + log2 l).
+// Taking the value scale into the exponent keeps p in (0, 1] whatever the scales are, so that it can be rounded to f16 (held
+// 2^15 times as large: normal down to 2^-29 of the largest): 2^-11 of a term where bf16 would lose 2^-8, on the same matrix
+// instruction.  Codes are whole numbers below 2^8 or e4m3 values, exact in bf16 and in f16, and enter the products
+// exactly; scales are applied to scores in fp32.  Q is exact too: bf16 rows multiply bf16 keys, f16 rows f16 keys; f32 rows are split
+// into three bf16 parts (24 bits) and their p into two f16 parts, each part one more product.
 //
 // Everything is computed transposed, S^T = K' Q^T and O^T = V'^T P^T, so that the tokens of a score tile are rows of the
-// accumulator and a probability is already in the lane that feeds it to the second product.  Which token a row of the first
-// product is, is free: row 4g + r of 16-token tile t of a 64-token block is token 16g + 4t + r.  Lane group g then holds the 16
-// consecutive tokens 16g .. 16g + 15 — of one page, with one scale — and reads its values as 16 consecutive codes of one
-// dimension: one 16-byte load from the [dim][token] order of the cache, no LDS and no exchange between lanes.
+// accumulator and a probability is already in the lane that feeds it to the second product: no exchange between lanes.
+// Which token a row of the first product is, is free; it is chosen so that a lane holds 16 consecutive tokens — of one page,
+// with one scale — and the matching piece of V' is 16 consecutive codes of one dimension in the cache's [dim][token] order.
+//
+// A page scale that is no finite number, or (where a mask cuts the tile) a NaN code among the values, must not reach rows
+// that do not see the token, and 0 * NaN is NaN: such values are taken as zeros and the token's score becomes NaN for the
+// rows that see it.
 #include <algorithm>
 #include "kvcache.hpp"
 
@@ -28,55 +32,115 @@ struct AttArgs {
     const char *q;
     char *out;
     int64_t q_row, q_head, o_row, o_head;
-    float *lse, *part_o, *part_ml;  // partials: [split][packed row][q head][dim] and [split][packed row][q head][2]
+    float *lse, *part_o, *part_ml;  // partials: [slice][packed row][q head][dim] and [slice][packed row][q head][2]
     float scale;                    // scale * log2(e)
-    int q_heads, group, causal, window, splits, row_tiles;
+    int q_heads, group, causal, window, splits, row_tiles, tile_rows;
 };
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 constexpr float kNone = -__builtin_inff();
+constexpr float kLift = 15.f;        // probabilities are held 2^15 times as large: at most 2^15 in f16, whose largest number is 65504
+constexpr float kTinyScale = 0x1p-100f;  // value scales below it are multiplied into the codes: 1 / scale stays finite
 
-// number of bf16 parts that hold a value of T for the products
-template <typename T> constexpr int kParts = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, f16_t> ? 2 : 3;
+// ---- products ---------------------------------------------------------------------------------------------------------
+// Kind: the 16-bit type of keys and queries; QP, PP: parts that hold a query value, a probability
+template <typename T> struct RowType { using Kind = __bf16; static constexpr int QP = 1, PP = 1; };
+template <> struct RowType<f16_t> { using Kind = _Float16; static constexpr int QP = 1, PP = 1; };
+template <> struct RowType<float> { using Kind = __bf16; static constexpr int QP = 3, PP = 2; };
 
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t)); }
-// eight values -> NP bf16 vectors whose sum they are (to 8 NP bits)
-template <int NP> __device__ __forceinline__ void split_parts(float (&x)[8], bf16x8 (&p)[NP]) {
+template <typename Kind> __device__ __forceinline__ f32x4_t mma16(const u32x4 &a, const u32x4 &b, const f32x4_t &c) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename Kind> __device__ __forceinline__ f32x16 mma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename Kind> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+// eight values -> N vectors of Kind whose sum they are, as far as N parts reach
+template <typename Kind, int N> __device__ __forceinline__ void split_parts(float (&x)[8], u32x4 (&p)[N]) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-        u32x4 w;
+    for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-            if (k + 1 < NP) {
-                x[2 * e] -= bits_to_float(w[e] << 16);
-                x[2 * e + 1] -= bits_to_float(w[e] & 0xffff0000u);
+            const uint32_t w = pack2<Kind>(x[2 * e], x[2 * e + 1]);
+            p[k][e] = w;
+            if (k + 1 < N) {
+                if constexpr (std::is_same_v<Kind, __bf16>) {
+                    x[2 * e] -= bits_to_float(w << 16);
+                    x[2 * e + 1] -= bits_to_float(w & 0xffff0000u);
+                } else {
+                    const f16x2_t h = __builtin_bit_cast(f16x2_t, w);
+                    x[2 * e] -= (float)h[0];
+                    x[2 * e + 1] -= (float)h[1];
+                }
             }
         }
-        p[k] = __builtin_bit_cast(bf16x8, w);
+}
+// four codes (a dword) as Kind, exactly
+template <typename Code, typename Kind> __device__ __forceinline__ void codes4(uint32_t c, uint32_t &lo, uint32_t &hi) {
+    if constexpr (std::is_same_v<Code, CodeE4M3> && std::is_same_v<Kind, __bf16>) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
+    } else if constexpr (std::is_same_v<Code, CodeE4M3>) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, true));
+    } else if constexpr (std::is_same_v<Kind, _Float16>) {
+        // 0x6400 + u is 1024 + u in f16, u = code + 128 < 256: exact, and so is the difference
+        const uint32_t u = c ^ 0x80808080u;
+        const f16x2_t off = {(_Float16)1152.f, (_Float16)1152.f};
+        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+    } else {
+        float x[4];
+        Code::decode(c, x);
+        lo = pack2<Kind>(x[0], x[1]);
+        hi = pack2<Kind>(x[2], x[3]);
     }
 }
-// eight codes (two dwords) as bf16, exactly
-template <typename Code> __device__ __forceinline__ bf16x8 codes_bf16(uint32_t a, uint32_t b) {
-    u32x4 w;
-    if constexpr (std::is_same_v<Code, CodeE4M3>) {
-        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
-        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true));
-        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false));
-        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
-    } else {
-        float x[8];
-        Code::decode(a, x);
-        Code::decode(b, x + 4);
+template <typename Code, typename Kind> __device__ __forceinline__ u32x4 codes8(uint32_t a, uint32_t b) {
+    uint32_t w0, w1, w2, w3;
+    codes4<Code, Kind>(a, w0, w1);
+    codes4<Code, Kind>(b, w2, w3);
+    return u32x4{w0, w1, w2, w3};
+}
+// eight f16 values times f
+__device__ __forceinline__ u32x4 times(const u32x4 &v, float f) {
+    f16x8 x = __builtin_bit_cast(f16x8, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-    }
-    return __builtin_bit_cast(bf16x8, w);
+    for (int e = 0; e < 8; ++e) x[e] = (_Float16)((float)x[e] * f);
+    return __builtin_bit_cast(u32x4, x);
 }
 // bytes of `w` that are an e4m3 NaN, as 0x80 in each
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// 16 codes without their NaNs; bit j of the result: code j was one
+__device__ __forceinline__ uint32_t drop_nans(u32x4 &v) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t b = nan_bytes(v[w]);
+        v[w] &= ~((b >> 7) * 0xffu);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= ((b >> (8 * e + 7)) & 1u) << (4 * w + e);
+    }
+    return found;
+}
 
-// The tokens [lo, hi) that row r of a sequence sees; nothing for a row that is none or has no place in the cache.
+// A value scale: its logarithm and reciprocal, and what the codes are to be multiplied with (1 but for zero, tiny and negative
+// scales); `fine`: it is a finite number.
+struct ValueScale { float log, inv; };
+__device__ __forceinline__ ValueScale value_scale(float vs) {
+    const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
+    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag)};
+}
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
+__device__ __forceinline__ float code_factor(float vs) { return __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f; }
+
+// ---- which tokens -------------------------------------------------------------------------------------------------------
+// The tokens [lo, hi) that row i of a sequence sees; nothing for a row that is none or has no place in the cache.
 struct Range { int lo, hi; };
 __device__ __forceinline__ Range row_range(const AttArgs &a, const KvSeq &s, int i) {
     const int p = s.begin + i;
@@ -96,17 +160,54 @@ __device__ __forceinline__ void tile_range(const AttArgs &a, const KvSeq &s, int
     first = x.lo / 64;
     last = (y.hi + 63) / 64;
 }
-// the part of [first, last) that slice `split` of `splits` walks
-__device__ __forceinline__ void slice_of(int splits, int split, int &first, int &last) {
-    const int each = (last - first + splits - 1) / splits, b = first + split * each, e = b + each < last ? b + each : last;
-    first = b;
-    last = e;
+// tiles in a slice when `tiles` of them are cut into at most `splits` slices: no fewer than kMinTiles
+constexpr int kMinTiles = 8;
+__device__ __forceinline__ int slice_tiles(int tiles, int splits) {
+    const int each = (tiles + splits - 1) / splits;
+    return each < kMinTiles ? kMinTiles : each;
 }
+// the part of [first, last) that slice `split` walks; false if there is none (slice 0 always has one, if empty)
+__device__ __forceinline__ bool slice_of(const AttArgs &a, int split, int &first, int &last) {
+    const int each = a.splits > 1 ? slice_tiles(last - first, a.splits) : last - first, b = first + split * each;
+    last = b + each < last ? b + each : last;
+    first = b;
+    return split == 0 || first < last;
+}
+__device__ __forceinline__ int page_at(const AttArgs &a, const KvSeq &s, int seq, int token) {  // of a token below the length, else -1
+    return token < s.length ? (int)kv_page(a.kv, seq, token >> a.kv.page_shift) : -1;
+}
+// eight values of a row as Kind parts; zeros past the end of the head
+template <typename T, int QP> __device__ __forceinline__ void load_query(const T *src, bool there, u32x4 (&q)[QP]) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    if (there) {
+        constexpr int V = kVecBytes / (int)sizeof(T);
+#pragma unroll
+        for (int p = 0; p < 8 / V; ++p) {
+            const vec_t<T, V> w = reinterpret_cast<const vec_t<T, V> *>(src)[p];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[p * V + e] = load_acc(w.v[e]);
+        }
+    }
+    split_parts<typename RowType<T>::Kind, QP>(x, q);
+}
+template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, float x1, float x2, float x3) {
+    const float y[4] = {x0, x1, x2, x3};
+    vec_t<T, 4> w;
+    store_acc_vec<T, 4>(w, y);
+    *reinterpret_cast<vec_t<T, 4> *>(dst) = w;
+}
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? kNone : kLn2 * (m - kLift + __builtin_amdgcn_logf(l)); }
 
-// One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile.
+// ---- few rows -------------------------------------------------------------------------------------------------------------
+// One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile
+// and meet at the end.  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
+// loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes.
 template <typename T, typename Code, int SPANS>
-__global__ __launch_bounds__(kBlock) void kvattention_kernel(const AttArgs a) {
-    constexpr int NP = kParts<T>, DT = SPANS * 4;  // 16-dimension tiles of the padded head
+__global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
+    using Kind = typename RowType<T>::Kind;
+    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
     __shared__ float meet_o[2][16][SPANS * 64 + 4];
     __shared__ float meet_m[4][16], meet_l[4][16];
     unsigned blk = blockIdx.x;
@@ -120,108 +221,100 @@ __global__ __launch_bounds__(kBlock) void kvattention_kernel(const AttArgs a) {
     const int D = a.kv.dim, P = a.kv.page_size;
     int tile, tile_end;
     tile_range(a, s, r0 / G, (r0 + 15) / G, tile, tile_end);
-    slice_of(a.splits, split, tile, tile_end);
-    if (a.splits > 1 && tile >= tile_end && split > 0) return;  // the joining launch knows
+    if (!slice_of(a, split, tile, tile_end)) return;  // the joining launch knows
+
+    // keys: row n of score tile t is token 16 (n / 4) + 4 t + n % 4; values and scales: tokens 16 g .. 16 g + 15
+    const int kofs = 16 * (n >> 2), gofs = 16 * g;
+    tile += wave;
+    int kp = -1, gp = -1;
+    if (tile < tile_end) { kp = page_at(a, s, seq, tile * 64 + kofs); gp = page_at(a, s, seq, tile * 64 + gofs); }
 
     // this lane's row
     const int r = r0 + n, i = r / G, h = head * G + (r - i * G);
     const bool real = r < rows;
     Range vis = row_range(a, s, i);
     if (!real) vis = {0, 0};
-    bf16x8 q[SPANS * 2][NP];
+    u32x4 q[SPANS * 2][QP];
     {
         const T *src = (const T *)a.q + (s.first + i) * a.q_row + h * a.q_head;
 #pragma unroll
         for (int c = 0; c < SPANS * 2; ++c) {  // span c / 2, half c % 2
             const int d = (c / 2) * 64 + g * 16 + (c % 2) * 8;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-            if (real && d < D) {
-                constexpr int V = kVecBytes / (int)sizeof(T);
-#pragma unroll
-                for (int p = 0; p < 8 / V; ++p) {
-                    const vec_t<T, V> w = *reinterpret_cast<const vec_t<T, V> *>(src + d + p * V);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[p * V + e] = load_acc(w.v[e]);
-                }
-            }
-            split_parts<NP>(x, q[c]);
+            load_query<T, QP>(src + d, real && d < D, q[c]);
         }
     }
     // a tile needs no masks when every real row sees all of it
     const int last_row = (r0 + 15 < rows ? r0 + 15 : rows - 1) / G;
-    const Range first_vis = row_range(a, s, r0 / G), last_vis = row_range(a, s, last_row);
-    const int all_lo = last_vis.lo, all_hi = first_vis.hi;
+    const int all_lo = row_range(a, s, last_row).lo, all_hi = row_range(a, s, r0 / G).hi;
 
     float m = kNone, l = 0.f;
     f32x4_t o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (tile += wave; tile < tile_end; tile += 4) {
-        const int tok0 = tile * 64;
-        // keys: row n of score tile t is token 16 (n / 4) + 4 t + n % 4; values and scales: tokens 16 g .. 16 g + 15
-        const int kb = tok0 + 16 * (n >> 2), gb = tok0 + 16 * g;
-        const int64_t kp = kb < s.length ? kv_page(a.kv, seq, kb >> a.kv.page_shift) : -1;
-        const int64_t gp = gb < s.length ? kv_page(a.kv, seq, gb >> a.kv.page_shift) : -1;
+    for (; tile < tile_end; tile += 4) {
+        const int tok0 = tile * 64, gb = tok0 + gofs;
         u32x4 kc[4][SPANS], vc[DT];
+        const uint8_t *ksrc = a.kv.k + ((int64_t)kp * a.kv.heads + head) * P * D + (((tok0 + kofs) & (P - 1)) + (n & 3)) * D + g * 16;
+        const uint8_t *vsrc = a.kv.v + ((int64_t)gp * a.kv.heads + head) * P * D + n * P + (gb & (P - 1));
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < SPANS; ++c) {
                 kc[t][c] = u32x4{0u, 0u, 0u, 0u};
-                if (kp >= 0 && c * 64 + g * 16 < D)
-                    kc[t][c] = *reinterpret_cast<const u32x4 *>(a.kv.k + ((kp * a.kv.heads + head) * P + ((kb & (P - 1)) + 4 * t + (n & 3))) * D + c * 64 + g * 16);
+                if (kp >= 0 && c * 64 + g * 16 < D) kc[t][c] = *reinterpret_cast<const u32x4 *>(ksrc + 4 * t * D + c * 64);
             }
+        float ks = 0.f, vs = 0.f;
+        if (gp >= 0) {
+            ks = a.kv.k_scale[(int64_t)gp * a.kv.heads + head] * a.scale;
+            vs = a.kv.v_scale[(int64_t)gp * a.kv.heads + head];
+        }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             vc[t] = u32x4{0u, 0u, 0u, 0u};
-            if (gp >= 0 && t * 16 < D) vc[t] = *reinterpret_cast<const u32x4 *>(a.kv.v + ((gp * a.kv.heads + head) * D + (t * 16 + n)) * P + (gb & (P - 1)));
+            if (gp >= 0 && t * 16 < D) vc[t] = *reinterpret_cast<const u32x4 *>(vsrc + t * 16 * P);
         }
-        const float ks = gp >= 0 ? a.kv.k_scale[gp * a.kv.heads + head] * a.scale : 0.f;
-        const float vs = gp >= 0 ? a.kv.v_scale[gp * a.kv.heads + head] : 0.f;
-        const bool masked = tok0 < all_lo || tok0 + 64 > all_hi || __any(gp < 0);
+        const bool none = gp < 0, masked = tok0 < all_lo || tok0 + 64 > all_hi || __any(none);
+        if (tile + 4 < tile_end) { kp = page_at(a, s, seq, tok0 + 256 + kofs); gp = page_at(a, s, seq, tok0 + 256 + gofs); }
 
+        const ValueScale vsc = value_scale(vs);
+        const bool fine = finite(vs);
         float sc[16];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < SPANS * 2; ++c) {
-                const bf16x8 k = codes_bf16<Code>(kc[t][c / 2][(c % 2) * 2], kc[t][c / 2][(c % 2) * 2 + 1]);
+                const u32x4 k = codes8<Code, Kind>(kc[t][c / 2][(c % 2) * 2], kc[t][c / 2][(c % 2) * 2 + 1]);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c][p], acc, 0, 0, 0);
+                for (int p = 0; p < QP; ++p) acc = mma16<Kind>(k, q[c][p], acc);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[4 * t + e] = acc[e] * ks;
+            for (int e = 0; e < 4; ++e) sc[4 * t + e] = __builtin_fmaf(acc[e], ks, vsc.log);
         }
-        if (masked) {
+        if (masked || __any(!fine)) {
+            uint32_t bad = fine ? 0u : 0xffffu;  // bit j: the score of token 16 g + j becomes NaN
             if constexpr (std::is_same_v<Code, CodeE4M3>) {
-                // 0 * NaN is NaN: a NaN among the values of a token becomes 0 here and makes the token's score NaN for the rows that see it
-                uint32_t bad = 0, any = 0;  // bad: bit j = token 16 g + j
+                uint32_t any = 0;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) any |= nan_bytes(vc[t][w]);
-                if (__any(any != 0)) {
+                if (masked && __any(any != 0)) {
 #pragma unroll
-                    for (int t = 0; t < DT; ++t)
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t b = nan_bytes(vc[t][w]);
-                            vc[t][w] &= ~((b >> 7) * 0xffu);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) bad |= ((b >> (8 * e + 7)) & 1u) << (4 * w + e);
-                        }
+                    for (int t = 0; t < DT; ++t) bad |= drop_nans(vc[t]);
 #pragma unroll
                     for (int x = 1; x < 16; x <<= 1) bad |= __shfl_xor(bad, x, 16);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) if (bad >> e & 1u) sc[e] = __builtin_nanf("");
                 }
             }
+            if (!fine)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) if (gp < 0 || gb + e < vis.lo || gb + e >= vis.hi) sc[e] = kNone;
+                for (int t = 0; t < DT; ++t) vc[t] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (bad >> e & 1u) sc[e] = __builtin_nanf("");
+                if (none || gb + e < vis.lo || gb + e >= vis.hi) sc[e] = kNone;
+            }
         }
         float top = m;
 #pragma unroll
@@ -231,28 +324,30 @@ __global__ __launch_bounds__(kBlock) void kvattention_kernel(const AttArgs a) {
         const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
         m = top;
         float sum = 0.f;
-        bf16x8 p[2][NP];
+        u32x4 p[2][PP];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = __builtin_amdgcn_exp2f(sc[8 * u + e] - base);
-                sum += y;
-                x[e] = sc[8 * u + e] == kNone ? 0.f : y * vs;  // whatever the scale of a page nobody sees is
+                x[e] = __builtin_amdgcn_exp2f(sc[8 * u + e] - (base - kLift));
+                sum += x[e];
             }
-            split_parts<NP>(x, p[u]);
+            split_parts<_Float16, PP>(x, p[u]);
         }
-        l = l * alpha + sum;
+        l = __builtin_fmaf(sum, vsc.inv, l * alpha);
+        const float factor = code_factor(vs);
+        const bool plain = !__any(factor != 1.f);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             if (t * 16 < D) {
                 o[t] *= alpha;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const bf16x8 v = codes_bf16<Code>(vc[t][2 * u], vc[t][2 * u + 1]);
+                    u32x4 v = codes8<Code, _Float16>(vc[t][2 * u], vc[t][2 * u + 1]);
+                    if (!plain) v = times(v, fine ? factor : 1.f);
 #pragma unroll
-                    for (int k = 0; k < NP; ++k) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[u][k], o[t], 0, 0, 0);
+                    for (int k = 0; k < PP; ++k) o[t] = mma16<_Float16>(v, p[u][k], o[t]);
                 }
             }
         }
@@ -296,51 +391,332 @@ __global__ __launch_bounds__(kBlock) void kvattention_kernel(const AttArgs a) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-        if (t * 16 < D) {
-            float y[4];
-            vec_t<T, 4> w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = o[t][e] * inv;
-            store_acc_vec<T, 4>(w, y);
-            *reinterpret_cast<vec_t<T, 4> *>(dst + t * 16 + g * 4) = w;
-        }
-    }
-    if (g == 0 && a.lse) a.lse[at] = l == 0.f ? kNone : kLn2 * (top + __builtin_amdgcn_logf(l));
+    for (int t = 0; t < DT; ++t)
+        if (t * 16 < D) store4<T>(dst + t * 16 + g * 4, o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv);
+    if (g == 0 && a.lse) a.lse[at] = lse_of(top, l);
 }
 
-// Joins the slices of a row, in slice order: one workgroup of `dim` rounded up to 64 threads for each packed row slot of a sequence and head
+// ---- many rows ------------------------------------------------------------------------------------------------------------
+// One workgroup: 32 rows a wave of one (sequence, key head); the waves share every 64-token tile, whose codes are turned into
+// 16-bit operands once, on their way from registers (loaded a tile ahead) into LDS.  Scores: two 32-token products of
+// 32x32x16; row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
+// their probabilities to the second product as they are.  Rows of LDS are padded by 16 bytes: 16 lanes that read 16 bytes at
+// one column of 16 rows meet 16 different bank groups.  Bound by the matrix pipe and the vector pipe's 2^x.
+template <typename T, typename Code, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>::QP == 1) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
+    using Kind = typename RowType<T>::Kind;
+    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = DP / 32, THREADS = WAVES * kWave;
+    constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, PIECES = (DP * 4 + THREADS - 1) / THREADS;
+    __shared__ __attribute__((aligned(16))) unsigned char kl[64 * KPITCH], vl[DP * VPITCH];
+    __shared__ uint32_t bad_tokens[2][2];
+    // longest tiles of rows first; the tiles of one (sequence, head) stay on one XCD when there are a multiple of 8 pairs
+    const unsigned pairs = (unsigned)a.kv.batch * a.kv.heads;
+    unsigned blk = blockIdx.x;
+    const int pair = blk % pairs; blk /= pairs;
+    const int split = blk % (unsigned)a.splits, rt = a.row_tiles - 1 - (int)(blk / (unsigned)a.splits);
+    const int head = pair % a.kv.heads, seq = pair / a.kv.heads;
+    const KvSeq s = kv_seq(a.kv, seq);
+    const int G = a.group, rows = s.n * G, r0 = rt * (WAVES * 32);
+    if (r0 >= rows) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h2 = lane >> 5;
+    const int D = a.kv.dim, P = a.kv.page_size;
+    int tile, tile_end;
+    tile_range(a, s, r0 / G, (r0 + WAVES * 32 - 1) / G, tile, tile_end);
+    if (!slice_of(a, split, tile, tile_end)) return;
+
+    // pieces of 16 codes that this thread brings: of the keys token kt, dimensions kd ..; of the values dimension vd, tokens vt ..
+    int kt[PIECES], kd[PIECES], vd[PIECES], vt[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const int id = threadIdx.x + j * THREADS, per = D / 16;
+        const bool there = id < 4 * D;
+        kt[j] = there ? id / per : -1;
+        kd[j] = (id - (id / per) * per) * 16;
+        // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
+        vd[j] = !there ? -1 : P == 16 ? id % D : id >> 2;
+        vt[j] = (P == 16 ? id / D : id & 3) * 16;
+    }
+    if (threadIdx.x < 4) bad_tokens[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    if (D < DP) {  // what pads the head stays zero
+        for (int id = threadIdx.x; id < 64 * (DP - D) / 8; id += THREADS)
+            *reinterpret_cast<u32x4 *>(kl + (id / ((DP - D) / 8)) * KPITCH + D * 2 + (id % ((DP - D) / 8)) * 16) = u32x4{0u, 0u, 0u, 0u};
+        for (int id = threadIdx.x; id < (DP - D) * 8; id += THREADS) *reinterpret_cast<u32x4 *>(vl + (D + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+
+    // this lane's row
+    const int w0 = r0 + wave * 32, r = w0 + n, i = r / G, h = head * G + (r - i * G);
+    const bool real = r < rows;
+    Range vis = row_range(a, s, i);
+    if (!real) vis = {0, 0};
+    u32x4 q[DP / 16][QP];
+    {
+        const T *src = (const T *)a.q + (s.first + i) * a.q_row + h * a.q_head;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) load_query<T, QP>(src + c * 16 + h2 * 8, real && c * 16 < D, q[c]);
+    }
+    // tokens that any row of the wave sees, that all of them see; that all rows of the workgroup see
+    Range any = {0, 0}, all = {0, 0}, group_all;
+    {
+        const int last = (r0 + WAVES * 32 < rows ? r0 + WAVES * 32 : rows) - 1, wlast = w0 + 31 < rows ? w0 + 31 : rows - 1;
+        group_all = {row_range(a, s, last / G).lo, row_range(a, s, r0 / G).hi};
+        if (w0 < rows) {
+            const Range x = row_range(a, s, w0 / G), y = row_range(a, s, wlast / G);
+            any = {x.lo, y.hi};
+            all = {y.lo, x.hi};
+        }
+    }
+
+    float m = kNone, l = 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+
+    // page numbers two tiles ahead, codes and scales one
+    int kp[PIECES], vp[PIECES], sp[2];
+    u32x4 kc[PIECES], vc[PIECES];
+    float vcs[PIECES], ks_next[2], vs_next[2];
+    int sp_next[2];
+    auto pages = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            kp[j] = kt[j] < 0 ? -1 : page_at(a, s, seq, t * 64 + kt[j]);
+            vp[j] = vd[j] < 0 ? -1 : page_at(a, s, seq, t * 64 + vt[j]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sp[u] = page_at(a, s, seq, t * 64 + u * 32 + h2 * 16);
+    };
+    auto fetch = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            kc[j] = vc[j] = u32x4{0u, 0u, 0u, 0u};
+            vcs[j] = 1.f;
+            if (kp[j] >= 0) kc[j] = *reinterpret_cast<const u32x4 *>(a.kv.k + (((int64_t)kp[j] * a.kv.heads + head) * P + ((t * 64 + kt[j]) & (P - 1))) * D + kd[j]);
+            if (vp[j] >= 0) {
+                vc[j] = *reinterpret_cast<const u32x4 *>(a.kv.v + (((int64_t)vp[j] * a.kv.heads + head) * D + vd[j]) * P + ((t * 64 + vt[j]) & (P - 1)));
+                vcs[j] = a.kv.v_scale[(int64_t)vp[j] * a.kv.heads + head];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            sp_next[u] = sp[u];
+            ks_next[u] = vs_next[u] = 0.f;
+            if (sp[u] >= 0) {
+                ks_next[u] = a.kv.k_scale[(int64_t)sp[u] * a.kv.heads + head] * a.scale;
+                vs_next[u] = a.kv.v_scale[(int64_t)sp[u] * a.kv.heads + head];
+            }
+        }
+    };
+    if (tile < tile_end) {
+        pages(tile);
+        fetch(tile);
+        pages(tile + 1);
+    }
+    const int krow = (16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3)) * KPITCH + h2 * 16, vrow = n * VPITCH + h2 * 32;
+    __syncthreads();
+    for (; tile < tile_end; ++tile) {
+        const int tok0 = tile * 64, slot = tile & 1;
+        const bool group_masked = tok0 < group_all.lo || tok0 + 64 > group_all.hi;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            if (kt[j] >= 0) {
+                u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
+                dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
+                dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
+            }
+            if (vd[j] >= 0) {
+                u32x4 *dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
+                const bool fine = finite(vcs[j]);
+                if (!fine) vc[j] = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (std::is_same_v<Code, CodeE4M3>)
+                    if (group_masked) {
+                        const uint32_t found = drop_nans(vc[j]);
+                        if (found) atomicOr(&bad_tokens[slot][vt[j] >> 5], found << (vt[j] & 16));
+                    }
+                u32x4 x = codes8<Code, _Float16>(vc[j][0], vc[j][1]), y = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
+                const float f = code_factor(vcs[j]);
+                if (f != 1.f && fine) { x = times(x, f); y = times(y, f); }
+                dst[0] = x;
+                dst[1] = y;
+            }
+        }
+        float ks[2], vs[2];
+        int page[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) { ks[u] = ks_next[u]; vs[u] = vs_next[u]; page[u] = sp_next[u]; }
+        if (tile + 1 < tile_end) {
+            fetch(tile + 1);
+            pages(tile + 2);
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) bad_tokens[slot ^ 1][threadIdx.x] = 0;
+        if (tok0 < any.hi && tok0 + 64 > any.lo) {
+            f32x16 sc[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    const u32x4 k = *reinterpret_cast<const u32x4 *>(kl + krow + u * 32 * KPITCH + c * 32);
+#pragma unroll
+                    for (int p = 0; p < QP; ++p) sc[u] = mma32<Kind>(k, q[c][p], sc[u]);
+                }
+            }
+            const ValueScale vsc[2] = {value_scale(vs[0]), value_scale(vs[1])};
+            const uint32_t bad0 = bad_tokens[slot][0], bad1 = bad_tokens[slot][1];
+            const bool odd = tok0 < all.lo || tok0 + 64 > all.hi || (bad0 | bad1) ||
+                             __any(page[0] < 0 || page[1] < 0 || !(ks[0] >= 0.f) || !(ks[1] >= 0.f) || !finite(vs[0]) || !finite(vs[1]));
+            float top = m;
+            if (odd) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t bad = finite(vs[u]) ? (u ? bad1 : bad0) >> (16 * h2) : 0xffffu;
+                    const int t0 = tok0 + u * 32 + h2 * 16;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float x = __builtin_fmaf(sc[u][e], ks[u], vsc[u].log);
+                        if (bad >> e & 1u) x = __builtin_nanf("");
+                        if (page[u] < 0 || t0 + e < vis.lo || t0 + e >= vis.hi) x = kNone;
+                        sc[u][e] = x;
+                        top = __builtin_fmaxf(top, x);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x = sc[u][0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[u][e]);
+                    top = __builtin_fmaxf(top, __builtin_fmaf(x, ks[u], vsc[u].log));  // ks >= 0: the largest product is the largest score
+                }
+            }
+            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+            const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l *= alpha;
+            u32x4 p[2][2][PP];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // the scores are there already (mul 1, add 0) or still to be made from the products
+                const float mul = odd ? 1.f : ks[u], add = (odd ? 0.f : vsc[u].log) - (base - kLift);
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * v + e], mul, add));
+                        sum += x[e];
+                    }
+                    split_parts<_Float16, PP>(x, p[u][v]);
+                }
+                l = __builtin_fmaf(sum, vsc[u].inv, l);
+            }
+            if (__any(alpha != 1.f)) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[t] *= alpha;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + vrow + t * 32 * VPITCH + u * 64 + v * 16);
+#pragma unroll
+                        for (int k = 0; k < PP; ++k) o[t] = mma32<_Float16>(x, p[u][v][k], o[t]);
+                    }
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    if (!real) return;
+    const int64_t at = (s.first + i) * a.q_heads + h;
+    if (a.splits > 1) {
+        const int64_t slot = (int64_t)split * a.kv.rows * a.q_heads + at;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int d = t * 32 + b * 8 + h2 * 4;
+                if (d < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + d) = f32x4_t{o[t][4 * b], o[t][4 * b + 1], o[t][4 * b + 2], o[t][4 * b + 3]};
+            }
+        if (h2 == 0) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = t * 32 + b * 8 + h2 * 4;
+            if (d < D) store4<T>(dst + d, o[t][4 * b] * inv, o[t][4 * b + 1] * inv, o[t][4 * b + 2] * inv, o[t][4 * b + 3] * inv);
+        }
+    if (h2 == 0 && a.lse) a.lse[at] = lse_of(m, l);
+}
+
+// ---- the slices of a row ------------------------------------------------------------------------------------------------
+// One workgroup for a packed row and query head; a lane holds four dimensions, each wave adds every fourth slice, and the four
+// sums are added in wave order.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs a) {
+    __shared__ f32x4_t meet_o[3][kWave];
+    __shared__ float meet_l[3];
     unsigned blk = blockIdx.x;
     const int h = blk % (unsigned)a.q_heads; blk /= (unsigned)a.q_heads;
     const int i = blk % (unsigned)a.kv.max_rows, seq = blk / (unsigned)a.kv.max_rows;
     const KvSeq s = kv_seq(a.kv, seq);
     if (i >= s.n) return;
-    const int r0 = (i * a.group + h % a.group) / 16 * 16;
+    const int r0 = (i * a.group + h % a.group) / a.tile_rows * a.tile_rows;
     int first, last;
-    tile_range(a, s, r0 / a.group, (r0 + 15) / a.group, first, last);
-    const int each = (last - first + a.splits - 1) / a.splits, used = each > 0 ? (last - first + each - 1) / each : 1;
+    tile_range(a, s, r0 / a.group, (r0 + a.tile_rows - 1) / a.group, first, last);
+    const int each = slice_tiles(last - first, a.splits), used = last > first ? (last - first + each - 1) / each : 1;
     const int64_t at = (s.first + i) * a.q_heads + h, pitch = a.kv.rows * a.q_heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane * 4;
     float top = kNone;
-    for (int k = 0; k < used; ++k) top = __builtin_fmaxf(top, a.part_ml[2 * (at + k * pitch)]);
-    const float base = top == kNone ? 0.f : top;
-    float l = 0.f, o = 0.f;
-    const int d = threadIdx.x;
-    for (int k = 0; k < used; ++k) {
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + k * pitch)] - base);
-        l = __builtin_fmaf(w, a.part_ml[2 * (at + k * pitch) + 1], l);
-        if (d < a.kv.dim) o = __builtin_fmaf(w, a.part_o[(at + k * pitch) * a.kv.dim + d], o);
+    bool nan = false;
+    for (int k = lane; k < used; k += kWave) {
+        const float x = a.part_ml[2 * (at + k * pitch)];
+        nan = nan || x != x;
+        top = __builtin_fmaxf(top, x);
     }
-    if (d < a.kv.dim) ((T *)a.out)[(s.first + i) * a.o_row + h * a.o_head + d] = store_acc<T>(l == 0.f ? 0.f : o * (1.f / l));
-    if (d == 0 && a.lse) a.lse[at] = l == 0.f ? kNone : kLn2 * (top + __builtin_amdgcn_logf(l));
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+    const float base = top == kNone ? 0.f : top;
+    float l = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = wave; k < used; k += 4) {
+        const int64_t slot = at + k * pitch;
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * slot] - base);
+        l = __builtin_fmaf(w, a.part_ml[2 * slot + 1], l);
+        if (d < a.kv.dim) o += w * *reinterpret_cast<const f32x4_t *>(a.part_o + slot * a.kv.dim + d);
+    }
+    if (wave > 0) {
+        meet_o[wave - 1][lane] = o;
+        if (lane == 0) meet_l[wave - 1] = l;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) { l += meet_l[w]; o += meet_o[w][lane]; }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (d < a.kv.dim) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (lane == 0 && a.lse) a.lse[at] = lse_of(top, l);
 }
 
-// How many slices the tokens of a sequence are cut into: enough workgroups for the card, but at least four 64-token tiles
-// (one for each wave) a slice, counted on the longest sequence that the cache can hold.
-int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles) {
+// ---- launches -----------------------------------------------------------------------------------------------------------
+constexpr int kWaves = 4, kTileRows = kWaves * 32;
+constexpr int64_t kFewRows = 32;  // rows of one sequence and key head up to which the 16-row kernel runs
+
+// How many slices the tokens of a sequence are cut into: enough workgroups for the card, counted on the longest sequence that
+// the cache can hold; a slice has at least kMinTiles tiles (slice_tiles), so that short sequences use fewer.
+int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few) {
     const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles, tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
-    int64_t want = std::min<int64_t>((4 * kCUs + blocks - 1) / blocks, (tiles + 3) / 4);
+    int64_t want = std::min<int64_t>(((few ? 16 : 2) * kCUs + blocks - 1) / blocks, (tiles + kMinTiles - 1) / kMinTiles);
     const int64_t row_bytes = kv.rows * q_heads * (kv.dim + 2) * 4;
     want = std::min<int64_t>(want, ((int64_t)256 << 20) / std::max<int64_t>(1, row_bytes));  // partial results of at most 256 MiB
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
@@ -359,24 +735,31 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     a.group = q_heads / a.kv.heads;
     a.splits = 1;
     if (kv_nothing(a.kv)) return DXH_OK;
-    if ((int64_t)a.kv.max_rows * a.group > INT32_MAX - 64) return DXH_ERR_TOO_LARGE;
-    a.row_tiles = (int)(((int64_t)a.kv.max_rows * a.group + 15) / 16);
-    a.splits = choose_splits(a.kv, q_heads, a.row_tiles);
+    const int64_t most = (int64_t)a.kv.max_rows * a.group;
+    if (most > INT32_MAX - kTileRows) return DXH_ERR_TOO_LARGE;
+    a.tile_rows = most <= kFewRows ? 16 : kTileRows;
+    a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
+    a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16);
     if ((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits > INT32_MAX || (int64_t)a.kv.batch * a.kv.max_rows * q_heads > INT32_MAX) return DXH_ERR_TOO_LARGE;
     return DXH_OK;
 }
 
 template <typename T, typename Code> int launch(const AttArgs &a, hipStream_t st) {
     const unsigned blocks = (unsigned)((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits);
-    switch ((a.kv.dim + 63) / 64) {
-    case 1: kvattention_kernel<T, Code, 1><<<blocks, kBlock, 0, st>>>(a); break;
-    case 2: kvattention_kernel<T, Code, 2><<<blocks, kBlock, 0, st>>>(a); break;
-    case 3: kvattention_kernel<T, Code, 3><<<blocks, kBlock, 0, st>>>(a); break;
-    default: kvattention_kernel<T, Code, 4><<<blocks, kBlock, 0, st>>>(a); break;
+    if (a.tile_rows == 16) {
+        switch ((a.kv.dim + 63) / 64) {
+        case 1: kvattention_rows_kernel<T, Code, 1><<<blocks, kBlock, 0, st>>>(a); break;
+        case 2: kvattention_rows_kernel<T, Code, 2><<<blocks, kBlock, 0, st>>>(a); break;
+        default: kvattention_rows_kernel<T, Code, 4><<<blocks, kBlock, 0, st>>>(a); break;
+        }
+    } else {
+        if (a.kv.dim <= 64) kvattention_tiles_kernel<T, Code, 64, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+        else if (a.kv.dim <= 128) kvattention_tiles_kernel<T, Code, 128, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+        else kvattention_tiles_kernel<T, Code, 256, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
     }
     const int rc = launch_status();
     if (rc != DXH_OK || a.splits == 1) return rc;
-    kvattention_join_kernel<T><<<(unsigned)((int64_t)a.kv.batch * a.kv.max_rows * a.q_heads), (a.kv.dim + 63) / 64 * 64, 0, st>>>(a);
+    kvattention_join_kernel<T><<<(unsigned)((int64_t)a.kv.batch * a.kv.max_rows * a.q_heads), kBlock, 0, st>>>(a);
     return launch_status();
 }
 

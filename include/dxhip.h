@@ -574,9 +574,10 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * A row that sees no token gives zeros (lse: -infinity).  lse, if not NULL: [rows, q_heads] fp32, the natural logarithm of
  * the sum of exp(scale * q . k_j).  What tokens that a row does not see hold has no effect on it, NaN codes and scales of
  * pages without visible tokens included; a NaN among a visible token's values makes that dimension of the row, or the whole
- * row, NaN.  dtype f32 f16 bf16 for q and out (which must not overlap); q_heads a multiple of cache->heads.  Scores,
- * maxima, sums and the output are accumulated in fp32; a probability is rounded to bf16 for a bf16 row, kept to 16 bits of
- * precision for f16 and to 24 for f32; codes enter the products exactly.
+ * row, NaN, and so does a scale of a visible token's page that is not finite.  dtype f32 f16 bf16 for q and out (which must
+ * not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
+ * queries enter the products exactly; a probability is rounded to f16, held relative to the largest, for f16 and bf16 rows and
+ * kept to 22 bits for f32 rows.
  * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a
  * second launch: device memory of the caller of at least the query's bytes, 256-byte aligned, that no other call in flight
  * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows and q_heads alone; workspace may be NULL when it is 0. */

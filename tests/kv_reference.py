@@ -135,7 +135,7 @@ def attention(c, rows, q, scale, causal, window):
         lo = max(0, t - window + 1) if window else 0
         toks = [j for j in range(lo, hi) if c.page_of(b, j // c.page) >= 0]
         out, lse = np.zeros((q.shape[1], c.dim)), np.full(q.shape[1], -np.inf)
-        mag, big = np.zeros((q.shape[1], c.dim)), np.zeros(q.shape[1])
+        mag, big, weight = np.zeros((q.shape[1], c.dim)), np.zeros(q.shape[1]), np.zeros(q.shape[1])
         if toks:
             pg, at = np.array([c.page_of(b, j // c.page) for j in toks]), np.array(toks) % c.page
             K = decode(c.k[pg, :, at], c.code).astype(np.float64) * c.ks[pg].astype(np.float64)[..., None]
@@ -145,8 +145,9 @@ def attention(c, rows, q, scale, causal, window):
                 m = s.max()
                 e = np.exp(s - m)
                 out[h], lse[h] = e @ V[:, h // G] / e.sum(), m + np.log(e.sum())
+                weight[h] = (e * np.abs(c.vs[pg, h // G])).max() / e.sum()
                 mag[h], big[h] = e @ np.abs(V[:, h // G]) / e.sum(), (np.abs(K[:, h // G]) @ np.abs(q[r, h])).max() * abs(scale)
-        res[r] = (out, lse, mag, big, len(toks), np.abs(V).max() if toks else 0.0)
+        res[r] = (out, lse, mag, big, len(toks), np.abs(V).max() if toks else 0.0, weight)
     return res
 
 
@@ -156,13 +157,14 @@ def attention_bar(name, c, entry):
       products with scales: (D/32 + 40) u of scale sum|q||k|; f32 rows add 2^-24 of it for the split of q.
       probability: that as a relative error, the rounding of s - m (2 u |s - m|, |s - m| under twice the largest score) and of 2^x (4 u).
       sums over N tokens: (N/32 + 64) u.  Both the sum and its normalisation carry these: twice.
-      rounding of p * v_scale to 8, 16 or 24 bits: 2^-8, 2^-16, 2^-24 of sum p|v|; of the result: half a step.
+      rounding of p * v_scale to f16, or to two f16 parts for f32 rows: 2^-11, 2^-22 of sum p|v|; p * v_scale is held relative to its largest, 2^15
+      times as large, so that f16's smallest steps add at most 2^-25 2^-15 of the largest times a code for each token; of the result: half a step.
       underflow: the hardware's 2^x gives 0 below 2^-126, the smallest normal fp32 number; with l >= 1 (the largest term is 1) each of the N
       terms is off by at most 2^-126 max|v|."""
-    out, lse, mag, big, n, top = entry
+    out, lse, mag, big, n, top, weight = entry
     u = 2.0 ** -24
     s = ((c.dim / 32 + 42) * big + 4 * big + 4) * u
     sums = (n / 32 + 64) * u
-    part = {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[name]
-    bar = mag * (part + 2 * s + 2 * sums)[:, None] + np.abs(out) * HALF_STEP[name] * (1 + 2 ** -8) + TINY[name] + n * 2.0 ** -126 * top
+    part = {"bf16": 2.0 ** -11, "f16": 2.0 ** -11, "f32": 2.0 ** -22}[name]
+    bar = (n * 2.0 ** -40 * float(MAX[c.code]) * weight)[:, None] + mag * (part + 2 * s + 2 * sums)[:, None] + np.abs(out) * HALF_STEP[name] * (1 + 2 ** -8) + TINY[name] + n * 2.0 ** -126 * top
     return bar, s + sums + np.abs(np.where(np.isfinite(lse), lse, 0)) * 2 * u

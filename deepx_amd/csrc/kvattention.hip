@@ -107,13 +107,6 @@ template <typename Code, typename Kind> __device__ __forceinline__ u32x4 codes8(
     codes4<Code, Kind>(b, w2, w3);
     return u32x4{w0, w1, w2, w3};
 }
-// eight f16 values times f
-__device__ __forceinline__ u32x4 times(const u32x4 &v, float f) {
-    f16x8 x = __builtin_bit_cast(f16x8, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (_Float16)((float)x[e] * f);
-    return __builtin_bit_cast(u32x4, x);
-}
 // bytes of `w` that are an e4m3 NaN, as 0x80 in each
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // 16 codes without their NaNs; bit j of the result: code j was one
@@ -129,15 +122,15 @@ __device__ __forceinline__ uint32_t drop_nans(u32x4 &v) {
     return found;
 }
 
-// A value scale: its logarithm and reciprocal, and what the codes are to be multiplied with (1 but for zero, tiny and negative
-// scales); `fine`: it is a finite number.
-struct ValueScale { float log, inv; };
-__device__ __forceinline__ ValueScale value_scale(float vs) {
-    const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
-    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag)};
-}
 __device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
-__device__ __forceinline__ float code_factor(float vs) { return __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f; }
+// A value scale: its logarithm, its reciprocal, and the factor of the probabilities that go with it: 1 but for zero, tiny and
+// negative scales.  One that is not finite counts as 1 here and makes the scores of its tokens NaN.
+struct ValueScale { float log, inv, factor; };
+__device__ __forceinline__ ValueScale value_scale(float vs) {
+    if (!finite(vs)) vs = 1.f;
+    const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
+    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f};
+}
 
 // ---- which tokens -------------------------------------------------------------------------------------------------------
 // The tokens [lo, hi) that row i of a sequence sees; nothing for a row that is none or has no place in the cache.
@@ -173,8 +166,16 @@ __device__ __forceinline__ bool slice_of(const AttArgs &a, int split, int &first
     first = b;
     return split == 0 || first < last;
 }
-__device__ __forceinline__ int page_at(const AttArgs &a, const KvSeq &s, int seq, int token) {  // of a token below the length, else -1
-    return token < s.length ? (int)kv_page(a.kv, seq, token >> a.kv.page_shift) : -1;
+// The table's entry for a token, read without a branch (past the last page: the last page's), and the page it stands for: -1 if
+// the token is not below the length or the entry is none.  Loads go to page 0 then, which exists (a sequence of a cache without
+// pages has length 0), and what they bring is masked.
+__device__ __forceinline__ int entry_at(const AttArgs &a, int seq, int token) {
+    const int slot = token >> a.kv.page_shift, at = slot < a.kv.pages_per_seq ? slot : a.kv.pages_per_seq - 1;
+    const int64_t k = (int64_t)seq * a.kv.pages_per_seq + at;
+    return a.kv.table ? a.kv.table[k] : (int)k;
+}
+__device__ __forceinline__ int page_of(const AttArgs &a, const KvSeq &s, int entry, int token) {
+    return token < s.length && (unsigned)entry < (unsigned)a.kv.num_pages ? entry : -1;
 }
 // eight values of a row as Kind parts; zeros past the end of the head
 template <typename T, int QP> __device__ __forceinline__ void load_query(const T *src, bool there, u32x4 (&q)[QP]) {
@@ -204,8 +205,8 @@ __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? kN
 // One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile
 // and meet at the end.  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
 // loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes.
-template <typename T, typename Code, int SPANS>
-__global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
+template <typename T, typename Code, int SPANS, bool EXACT>
+__global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
     __shared__ float meet_o[2][16][SPANS * 64 + 4];
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
     const int G = a.group, rows = s.n * G, r0 = rt * 16;
     if (r0 >= rows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int D = a.kv.dim, P = a.kv.page_size;
+    const int D = EXACT ? SPANS * 64 : a.kv.dim, P = a.kv.page_size;
     int tile, tile_end;
     tile_range(a, s, r0 / G, (r0 + 15) / G, tile, tile_end);
     if (!slice_of(a, split, tile, tile_end)) return;  // the joining launch knows
@@ -226,8 +227,39 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
     // keys: row n of score tile t is token 16 (n / 4) + 4 t + n % 4; values and scales: tokens 16 g .. 16 g + 15
     const int kofs = 16 * (n >> 2), gofs = 16 * g;
     tile += wave;
-    int kp = -1, gp = -1;
-    if (tile < tile_end) { kp = page_at(a, s, seq, tile * 64 + kofs); gp = page_at(a, s, seq, tile * 64 + gofs); }
+    u32x4 kc[4][SPANS], vc[DT];
+    int kentry = 0, gentry = 0, gp = -1;
+    float ks = 0.f, vs = 0.f;
+    auto entries = [&](int t) __attribute__((always_inline)) { kentry = entry_at(a, seq, t * 64 + kofs); gentry = entry_at(a, seq, t * 64 + gofs); };
+    auto load_keys = [&](int t) __attribute__((always_inline)) {  // and the scales
+        const int k = page_of(a, s, kentry, t * 64 + kofs);
+        gp = page_of(a, s, gentry, t * 64 + gofs);
+        const uint8_t *src = a.kv.k + ((int64_t)(k < 0 ? 0 : k) * a.kv.heads + head) * P * D + (((t * 64 + kofs) & (P - 1)) + (n & 3)) * D;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < SPANS; ++c) {
+                const int d = c * 64 + g * 16;  // past the end of the head the query is zero: any key of the row will do
+                kc[u][c] = *reinterpret_cast<const u32x4 *>(src + 4 * u * D + (EXACT || d < D ? d : 0));
+            }
+        const int64_t at = (int64_t)(gp < 0 ? 0 : gp) * a.kv.heads + head;
+        ks = a.kv.k_scale[at];
+        vs = a.kv.v_scale[at];
+    };
+    auto load_values = [&](int t, int page) __attribute__((always_inline)) {
+        const uint8_t *src = a.kv.v + ((int64_t)(page < 0 ? 0 : page) * a.kv.heads + head) * P * D + ((t * 64 + gofs) & (P - 1));
+#pragma unroll
+        for (int u = 0; u < DT; ++u) {
+            const int d = u * 16 + n;  // dimensions past the end of the head are not stored
+            vc[u] = *reinterpret_cast<const u32x4 *>(src + (EXACT || d < D ? d : n) * P);
+        }
+    };
+    if (tile < tile_end) {
+        entries(tile);
+        load_keys(tile);
+        load_values(tile, gp);
+        entries(tile + 4);
+    }
 
     // this lane's row
     const int r = r0 + n, i = r / G, h = head * G + (r - i * G);
@@ -254,31 +286,10 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
 
     for (; tile < tile_end; tile += 4) {
         const int tok0 = tile * 64, gb = tok0 + gofs;
-        u32x4 kc[4][SPANS], vc[DT];
-        const uint8_t *ksrc = a.kv.k + ((int64_t)kp * a.kv.heads + head) * P * D + (((tok0 + kofs) & (P - 1)) + (n & 3)) * D + g * 16;
-        const uint8_t *vsrc = a.kv.v + ((int64_t)gp * a.kv.heads + head) * P * D + n * P + (gb & (P - 1));
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int c = 0; c < SPANS; ++c) {
-                kc[t][c] = u32x4{0u, 0u, 0u, 0u};
-                if (kp >= 0 && c * 64 + g * 16 < D) kc[t][c] = *reinterpret_cast<const u32x4 *>(ksrc + 4 * t * D + c * 64);
-            }
-        float ks = 0.f, vs = 0.f;
-        if (gp >= 0) {
-            ks = a.kv.k_scale[(int64_t)gp * a.kv.heads + head] * a.scale;
-            vs = a.kv.v_scale[(int64_t)gp * a.kv.heads + head];
-        }
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            vc[t] = u32x4{0u, 0u, 0u, 0u};
-            if (gp >= 0 && t * 16 < D) vc[t] = *reinterpret_cast<const u32x4 *>(vsrc + t * 16 * P);
-        }
-        const bool none = gp < 0, masked = tok0 < all_lo || tok0 + 64 > all_hi || __any(none);
-        if (tile + 4 < tile_end) { kp = page_at(a, s, seq, tok0 + 256 + kofs); gp = page_at(a, s, seq, tok0 + 256 + gofs); }
-
         const ValueScale vsc = value_scale(vs);
-        const bool fine = finite(vs);
+        const bool none = gp < 0, fine = finite(vs), more = tile + 4 < tile_end;
+        const float mul = ks * a.scale;
+        const bool odd = tok0 < all_lo || tok0 + 64 > all_hi || __any(none || !fine);
         float sc[16];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -290,9 +301,11 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
                 for (int p = 0; p < QP; ++p) acc = mma16<Kind>(k, q[c][p], acc);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[4 * t + e] = __builtin_fmaf(acc[e], ks, vsc.log);
+            for (int e = 0; e < 4; ++e) sc[4 * t + e] = __builtin_fmaf(acc[e], mul, vsc.log);
         }
-        if (masked || __any(!fine)) {
+        // the keys' registers are free: the next tile's keys come while this one's values are used
+        if (more) load_keys(tile + 4);
+        if (odd) {
             uint32_t bad = fine ? 0u : 0xffffu;  // bit j: the score of token 16 g + j becomes NaN
             if constexpr (std::is_same_v<Code, CodeE4M3>) {
                 uint32_t any = 0;
@@ -300,16 +313,16 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
                 for (int t = 0; t < DT; ++t)
 #pragma unroll
                     for (int w = 0; w < 4; ++w) any |= nan_bytes(vc[t][w]);
-                if (masked && __any(any != 0)) {
+                if (__any(any != 0)) {
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) bad |= drop_nans(vc[t]);
+                    for (int t = 0; t < DT; ++t) {
+                        const uint32_t found = drop_nans(vc[t]);
+                        if (EXACT || t * 16 < D) bad |= found;
+                    }
 #pragma unroll
                     for (int x = 1; x < 16; x <<= 1) bad |= __shfl_xor(bad, x, 16);
                 }
             }
-            if (!fine)
-#pragma unroll
-                for (int t = 0; t < DT; ++t) vc[t] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 if (bad >> e & 1u) sc[e] = __builtin_nanf("");
@@ -332,24 +345,24 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
             for (int e = 0; e < 8; ++e) {
                 x[e] = __builtin_amdgcn_exp2f(sc[8 * u + e] - (base - kLift));
                 sum += x[e];
+                x[e] *= vsc.factor;
             }
             split_parts<_Float16, PP>(x, p[u]);
         }
         l = __builtin_fmaf(sum, vsc.inv, l * alpha);
-        const float factor = code_factor(vs);
-        const bool plain = !__any(factor != 1.f);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            if (t * 16 < D) {
-                o[t] *= alpha;
+            o[t] *= alpha;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    u32x4 v = codes8<Code, _Float16>(vc[t][2 * u], vc[t][2 * u + 1]);
-                    if (!plain) v = times(v, fine ? factor : 1.f);
+            for (int u = 0; u < 2; ++u) {
+                const u32x4 v = codes8<Code, _Float16>(vc[t][2 * u], vc[t][2 * u + 1]);
 #pragma unroll
-                    for (int k = 0; k < PP; ++k) o[t] = mma16<_Float16>(v, p[u][k], o[t]);
-                }
+                for (int k = 0; k < PP; ++k) o[t] = mma16<_Float16>(v, p[u][k], o[t]);
             }
+        }
+        if (more) {
+            load_values(tile + 4, gp);
+            entries(tile + 8);
         }
     }
 
@@ -402,7 +415,7 @@ __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : RowType<T>::QP > 1 ? 2 : 3
 // 32x32x16; row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
 // their probabilities to the second product as they are.  Rows of LDS are padded by 16 bytes: 16 lanes that read 16 bytes at
 // one column of 16 rows meet 16 different bank groups.  Bound by the matrix pipe and the vector pipe's 2^x.
-template <typename T, typename Code, int DP, int WAVES>
+template <typename T, typename Code, int DP, bool EXACT, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>::QP == 1) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = DP / 32, THREADS = WAVES * kWave;
@@ -419,22 +432,24 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
     const int G = a.group, rows = s.n * G, r0 = rt * (WAVES * 32);
     if (r0 >= rows) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h2 = lane >> 5;
-    const int D = a.kv.dim, P = a.kv.page_size;
+    const int D = EXACT ? DP : a.kv.dim, P = a.kv.page_size;
     int tile, tile_end;
     tile_range(a, s, r0 / G, (r0 + WAVES * 32 - 1) / G, tile, tile_end);
     if (!slice_of(a, split, tile, tile_end)) return;
 
     // pieces of 16 codes that this thread brings: of the keys token kt, dimensions kd ..; of the values dimension vd, tokens vt ..
     int kt[PIECES], kd[PIECES], vd[PIECES], vt[PIECES];
+    bool there[PIECES];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const int id = threadIdx.x + j * THREADS, per = D / 16;
-        const bool there = id < 4 * D;
-        kt[j] = there ? id / per : -1;
-        kd[j] = (id - (id / per) * per) * 16;
+        there[j] = EXACT || id < 4 * D;  // others load piece 0 and drop it
+        const int x = there[j] ? id : 0;
+        kt[j] = x / per;
+        kd[j] = (x - kt[j] * per) * 16;
         // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
-        vd[j] = !there ? -1 : P == 16 ? id % D : id >> 2;
-        vt[j] = (P == 16 ? id / D : id & 3) * 16;
+        vd[j] = P == 16 ? x % D : x >> 2;
+        vt[j] = (P == 16 ? x / D : x & 3) * 16;
     }
     if (threadIdx.x < 4) bad_tokens[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     if (D < DP) {  // what pads the head stays zero
@@ -473,45 +488,40 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
 
-    // page numbers two tiles ahead, codes and scales one
-    int kp[PIECES], vp[PIECES], sp[2];
+    // table entries two tiles ahead, codes and scales one
+    int kentry[PIECES], ventry[PIECES], sentry[2], sp[2];
+    bool vnone[PIECES];
     u32x4 kc[PIECES], vc[PIECES];
-    float vcs[PIECES], ks_next[2], vs_next[2];
-    int sp_next[2];
-    auto pages = [&](int t) __attribute__((always_inline)) {
+    float ks_next[2], vs_next[2];
+    auto entries = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            kp[j] = kt[j] < 0 ? -1 : page_at(a, s, seq, t * 64 + kt[j]);
-            vp[j] = vd[j] < 0 ? -1 : page_at(a, s, seq, t * 64 + vt[j]);
+            kentry[j] = entry_at(a, seq, t * 64 + kt[j]);
+            ventry[j] = entry_at(a, seq, t * 64 + vt[j]);
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) sp[u] = page_at(a, s, seq, t * 64 + u * 32 + h2 * 16);
+        for (int u = 0; u < 2; ++u) sentry[u] = entry_at(a, seq, t * 64 + u * 32 + h2 * 16);
     };
     auto fetch = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            kc[j] = vc[j] = u32x4{0u, 0u, 0u, 0u};
-            vcs[j] = 1.f;
-            if (kp[j] >= 0) kc[j] = *reinterpret_cast<const u32x4 *>(a.kv.k + (((int64_t)kp[j] * a.kv.heads + head) * P + ((t * 64 + kt[j]) & (P - 1))) * D + kd[j]);
-            if (vp[j] >= 0) {
-                vc[j] = *reinterpret_cast<const u32x4 *>(a.kv.v + (((int64_t)vp[j] * a.kv.heads + head) * D + vd[j]) * P + ((t * 64 + vt[j]) & (P - 1)));
-                vcs[j] = a.kv.v_scale[(int64_t)vp[j] * a.kv.heads + head];
-            }
+            const int kp = page_of(a, s, kentry[j], t * 64 + kt[j]), vp = page_of(a, s, ventry[j], t * 64 + vt[j]);
+            vnone[j] = vp < 0;
+            kc[j] = *reinterpret_cast<const u32x4 *>(a.kv.k + (((int64_t)(kp < 0 ? 0 : kp) * a.kv.heads + head) * P + ((t * 64 + kt[j]) & (P - 1))) * D + kd[j]);
+            vc[j] = *reinterpret_cast<const u32x4 *>(a.kv.v + (((int64_t)(vp < 0 ? 0 : vp) * a.kv.heads + head) * D + vd[j]) * P + ((t * 64 + vt[j]) & (P - 1)));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            sp_next[u] = sp[u];
-            ks_next[u] = vs_next[u] = 0.f;
-            if (sp[u] >= 0) {
-                ks_next[u] = a.kv.k_scale[(int64_t)sp[u] * a.kv.heads + head] * a.scale;
-                vs_next[u] = a.kv.v_scale[(int64_t)sp[u] * a.kv.heads + head];
-            }
+            sp[u] = page_of(a, s, sentry[u], t * 64 + u * 32 + h2 * 16);
+            const int64_t at = (int64_t)(sp[u] < 0 ? 0 : sp[u]) * a.kv.heads + head;
+            ks_next[u] = a.kv.k_scale[at];
+            vs_next[u] = a.kv.v_scale[at];
         }
     };
     if (tile < tile_end) {
-        pages(tile);
+        entries(tile);
         fetch(tile);
-        pages(tile + 1);
+        entries(tile + 1);
     }
     const int krow = (16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3)) * KPITCH + h2 * 16, vrow = n * VPITCH + h2 * 32;
     __syncthreads();
@@ -520,34 +530,28 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
         const bool group_masked = tok0 < group_all.lo || tok0 + 64 > group_all.hi;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            if (kt[j] >= 0) {
-                u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
-                dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
-                dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
+            if (!there[j]) continue;
+            u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
+            dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
+            dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
+            if constexpr (std::is_same_v<Code, CodeE4M3>) {
+                if (vnone[j]) vc[j] = u32x4{0u, 0u, 0u, 0u};
+                if (group_masked) {
+                    const uint32_t found = drop_nans(vc[j]);
+                    if (found) atomicOr(&bad_tokens[slot][vt[j] >> 5], found << (vt[j] & 16));
+                }
             }
-            if (vd[j] >= 0) {
-                u32x4 *dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
-                const bool fine = finite(vcs[j]);
-                if (!fine) vc[j] = u32x4{0u, 0u, 0u, 0u};
-                if constexpr (std::is_same_v<Code, CodeE4M3>)
-                    if (group_masked) {
-                        const uint32_t found = drop_nans(vc[j]);
-                        if (found) atomicOr(&bad_tokens[slot][vt[j] >> 5], found << (vt[j] & 16));
-                    }
-                u32x4 x = codes8<Code, _Float16>(vc[j][0], vc[j][1]), y = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
-                const float f = code_factor(vcs[j]);
-                if (f != 1.f && fine) { x = times(x, f); y = times(y, f); }
-                dst[0] = x;
-                dst[1] = y;
-            }
+            dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
+            dst[0] = codes8<Code, _Float16>(vc[j][0], vc[j][1]);
+            dst[1] = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
         }
         float ks[2], vs[2];
         int page[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) { ks[u] = ks_next[u]; vs[u] = vs_next[u]; page[u] = sp_next[u]; }
+        for (int u = 0; u < 2; ++u) { ks[u] = ks_next[u] * a.scale; vs[u] = vs_next[u]; page[u] = sp[u]; }
         if (tile + 1 < tile_end) {
             fetch(tile + 1);
-            pages(tile + 2);
+            entries(tile + 2);
         }
         __syncthreads();
         if (threadIdx.x < 2) bad_tokens[slot ^ 1][threadIdx.x] = 0;
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
             const ValueScale vsc[2] = {value_scale(vs[0]), value_scale(vs[1])};
             const uint32_t bad0 = bad_tokens[slot][0], bad1 = bad_tokens[slot][1];
             const bool odd = tok0 < all.lo || tok0 + 64 > all.hi || (bad0 | bad1) ||
-                             __any(page[0] < 0 || page[1] < 0 || !(ks[0] >= 0.f) || !(ks[1] >= 0.f) || !finite(vs[0]) || !finite(vs[1]));
+                             __any(page[0] < 0 || page[1] < 0 || !(ks[0] >= 0.f) || !(ks[1] >= 0.f) || !finite(vs[0]) || !finite(vs[1]) || vsc[0].factor != 1.f || vsc[1].factor != 1.f);
             float top = m;
             if (odd) {
 #pragma unroll
@@ -610,6 +614,9 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
                         x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * v + e], mul, add));
                         sum += x[e];
                     }
+                    if (odd)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] *= vsc[u].factor;
                     split_parts<_Float16, PP>(x, p[u][v]);
                 }
                 l = __builtin_fmaf(sum, vsc[u].inv, l);
@@ -744,18 +751,20 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     return DXH_OK;
 }
 
-template <typename T, typename Code> int launch(const AttArgs &a, hipStream_t st) {
+template <typename T, typename Code, int SPANS, bool EXACT> void launch_dim(const AttArgs &a, hipStream_t st) {
     const unsigned blocks = (unsigned)((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits);
-    if (a.tile_rows == 16) {
-        switch ((a.kv.dim + 63) / 64) {
-        case 1: kvattention_rows_kernel<T, Code, 1><<<blocks, kBlock, 0, st>>>(a); break;
-        case 2: kvattention_rows_kernel<T, Code, 2><<<blocks, kBlock, 0, st>>>(a); break;
-        default: kvattention_rows_kernel<T, Code, 4><<<blocks, kBlock, 0, st>>>(a); break;
-        }
-    } else {
-        if (a.kv.dim <= 64) kvattention_tiles_kernel<T, Code, 64, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
-        else if (a.kv.dim <= 128) kvattention_tiles_kernel<T, Code, 128, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
-        else kvattention_tiles_kernel<T, Code, 256, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+    if (a.tile_rows == 16) kvattention_rows_kernel<T, Code, SPANS, EXACT><<<blocks, kBlock, 0, st>>>(a);
+    else kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+}
+template <typename T, typename Code> int launch(const AttArgs &a, hipStream_t st) {
+    switch (a.kv.dim) {  // head sizes that fill their registers need no bounds in the loops
+    case 64: launch_dim<T, Code, 1, true>(a, st); break;
+    case 128: launch_dim<T, Code, 2, true>(a, st); break;
+    case 256: launch_dim<T, Code, 4, true>(a, st); break;
+    default:
+        if (a.kv.dim < 64) launch_dim<T, Code, 1, false>(a, st);
+        else if (a.kv.dim < 128) launch_dim<T, Code, 2, false>(a, st);
+        else launch_dim<T, Code, 4, false>(a, st);
     }
     const int rc = launch_status();
     if (rc != DXH_OK || a.splits == 1) return rc;

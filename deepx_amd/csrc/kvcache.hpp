@@ -98,6 +98,7 @@ inline int kv_check(const dxh_kvcache *c, const dxh_kvrows *r, int dtype, KvArgs
     a.pages_per_seq = c->pages_per_seq; a.page_size = c->page_size; a.heads = c->heads; a.dim = c->dim;
     a.page_shift = __builtin_ctz((unsigned)c->page_size);
     a.batch = r->batch; a.max_rows = r->max_rows;
+    if (a.num_pages == 0) a.pages_per_seq = 0;  // no token has a place
     if (r->batch == 0 || r->rows == 0 || r->max_rows == 0) return DXH_OK;
     if (!r->lengths) return DXH_ERR_ARG;
     if (c->num_pages > 0 && c->pages_per_seq > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return DXH_ERR_ARG;

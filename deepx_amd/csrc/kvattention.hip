@@ -154,7 +154,7 @@ __device__ __forceinline__ void tile_range(const AttArgs &a, const KvSeq &s, int
     last = (y.hi + 63) / 64;
 }
 // tiles in a slice when `tiles` of them are cut into at most `splits` slices: no fewer than kMinTiles
-constexpr int kMinTiles = 8;
+constexpr int kMinTiles = 16;
 __device__ __forceinline__ int slice_tiles(int tiles, int splits) {
     const int each = (tiles + splits - 1) / splits;
     return each < kMinTiles ? kMinTiles : each;
@@ -666,12 +666,12 @@ __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>
 }
 
 // ---- the slices of a row ------------------------------------------------------------------------------------------------
-// One workgroup for a packed row and query head; a lane holds four dimensions, each wave adds every fourth slice, and the four
-// sums are added in wave order.
+// One workgroup for a packed row and query head.  Groups of dim / 4 lanes (rounded up to a power of two) take every so many-th
+// slice, each in one pass with a running maximum, and meet in LDS; the group's sums are added in group order.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs a) {
-    __shared__ f32x4_t meet_o[3][kWave];
-    __shared__ float meet_l[3];
+    __shared__ f32x4_t meet_o[kBlock];
+    __shared__ float meet_m[16], meet_l[16];
     unsigned blk = blockIdx.x;
     const int h = blk % (unsigned)a.q_heads; blk /= (unsigned)a.q_heads;
     const int i = blk % (unsigned)a.kv.max_rows, seq = blk / (unsigned)a.kv.max_rows;
@@ -682,48 +682,51 @@ __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs 
     tile_range(a, s, r0 / a.group, (r0 + a.tile_rows - 1) / a.group, first, last);
     const int each = slice_tiles(last - first, a.splits), used = last > first ? (last - first + each - 1) / each : 1;
     const int64_t at = (s.first + i) * a.q_heads + h, pitch = a.kv.rows * a.q_heads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane * 4;
-    float top = kNone;
-    bool nan = false;
-    for (int k = lane; k < used; k += kWave) {
-        const float x = a.part_ml[2 * (at + k * pitch)];
-        nan = nan || x != x;
-        top = __builtin_fmaxf(top, x);
-    }
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
-    const float base = top == kNone ? 0.f : top;
-    float l = 0.f;
+    const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64, groups = kBlock / lanes, group = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
+    const bool live = d < a.kv.dim;
+    const float *po = a.part_o + at * a.kv.dim + (live ? d : 0), *pm = a.part_ml + 2 * at;
+    float m = kNone, l = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int k = wave; k < used; k += 4) {
-        const int64_t slot = at + k * pitch;
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * slot] - base);
-        l = __builtin_fmaf(w, a.part_ml[2 * slot + 1], l);
-        if (d < a.kv.dim) o += w * *reinterpret_cast<const f32x4_t *>(a.part_o + slot * a.kv.dim + d);
+    for (int k = group; k < used; k += groups) {
+        const f32x4_t x = *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim);
+        const float mk = pm[2 * k * pitch], lk = pm[2 * k * pitch + 1];
+        const float top = __builtin_fmaxf(m, mk), base = top == kNone ? 0.f : top;
+        const float wa = __builtin_amdgcn_exp2f(m - base), wb = __builtin_amdgcn_exp2f(mk - base);
+        o = o * wa + x * wb;
+        l = __builtin_fmaf(l, wa, lk * wb);
+        m = top;
     }
-    if (wave > 0) {
-        meet_o[wave - 1][lane] = o;
-        if (lane == 0) meet_l[wave - 1] = l;
-    }
+    meet_o[threadIdx.x] = o;
+    if (threadIdx.x % lanes == 0) { meet_m[group] = m; meet_l[group] = l; }
     __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < 3; ++w) { l += meet_l[w]; o += meet_o[w][lane]; }
+    if (group > 0) return;
+    float top = m;
+    for (int k = 1; k < groups; ++k) top = __builtin_fmaxf(top, meet_m[k]);
+    const float base = top == kNone ? 0.f : top;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+    for (int k = 0; k < groups; ++k) {
+        const float w = __builtin_amdgcn_exp2f(meet_m[k] - base);
+        o += meet_o[k * lanes + threadIdx.x] * w;
+        l = __builtin_fmaf(meet_l[k], w, l);
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (d < a.kv.dim) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (lane == 0 && a.lse) a.lse[at] = lse_of(top, l);
+    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (threadIdx.x == 0 && a.lse) a.lse[at] = lse_of(top, l);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 constexpr int kWaves = 4, kTileRows = kWaves * 32;
 constexpr int64_t kFewRows = 32;  // rows of one sequence and key head up to which the 16-row kernel runs
 
-// How many slices the tokens of a sequence are cut into: enough workgroups for the card, counted on the longest sequence that
-// the cache can hold; a slice has at least kMinTiles tiles (slice_tiles), so that short sequences use fewer.
+// How many slices the tokens of a sequence are cut into, counted on the longest sequence that the cache can hold; a slice has at
+// least kMinTiles tiles (slice_tiles), so that short sequences use fewer.  The sequences of a batch differ in length: 8
+// workgroups a CU let the card fill the gaps that short ones leave (64 sequences of 1k-16k tokens: 245 us at 4, 229 at 8, 230
+// at 16); one sequence is cut into what runs at once, two workgroups a CU (131071 tokens: 64 us at 2, 76 at 4).
 int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few) {
     const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles, tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
-    int64_t want = std::min<int64_t>(((few ? 16 : 2) * kCUs + blocks - 1) / blocks, (tiles + kMinTiles - 1) / kMinTiles);
+    int64_t want = std::min<int64_t>(((few && kv.batch > 1 ? 8 : 2) * kCUs + blocks - 1) / blocks, (tiles + kMinTiles - 1) / kMinTiles);
     const int64_t row_bytes = kv.rows * q_heads * (kv.dim + 2) * 4;
     want = std::min<int64_t>(want, ((int64_t)256 << 20) / std::max<int64_t>(1, row_bytes));  // partial results of at most 256 MiB
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));

@@ -66,6 +66,7 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
 
     float top = 0.f;
     const int per_row = D / V, pieces = (t1 - t0) * per_row;
+#pragma unroll 4
     for (int i = threadIdx.x; i < pieces; i += THREADS) {
         const int r = i / per_row, d = (i - r * per_row) * V;
         const vec_t<T, V> q = *reinterpret_cast<const vec_t<T, V> *>(x + r * pitch + d);
@@ -98,12 +99,14 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
                 }
             } else {
                 const T *src = x + (t - t0) * pitch + d;
+                vec_t<T, V> r[16 / V];
+#pragma unroll
+                for (int q = 0; q < 16 / V; ++q) r[q] = reinterpret_cast<const vec_t<T, V> *>(src)[q];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const vec_t<T, 4> r = reinterpret_cast<const vec_t<T, 4> *>(src)[q];
                     float y[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = code_value<Code>(load_acc(r.v[e]), inv);
+                    for (int e = 0; e < 4; ++e) y[e] = code_value<Code>(load_acc(r[(4 * q + e) / V].v[(4 * q + e) % V]), inv);
                     w[q] = Code::encode(y);
                 }
             }
@@ -117,6 +120,13 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
             u32x4 *dst = reinterpret_cast<u32x4 *>(codes + d * P + t);
             const bool all_new = t >= t0 && t + 16 <= t1;
             u32x4 w = {0u, 0u, 0u, 0u};
+            // all 16 loads at once, those of tokens that are not new from the nearest new one
+            T r[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int tt = t + e < t0 ? t0 : t + e >= t1 ? t1 - 1 : t + e;
+                r[e] = x[(tt - t0) * pitch + d];
+            }
             if (!all_new) w = *dst;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -125,10 +135,8 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int tt = t + 4 * q + e;
-                    const bool fresh = tt >= t0 && tt < t1;
-                    y[e] = 0.f;
-                    if (fresh) y[e] = code_value<Code>(load_acc(x[(tt - t0) * pitch + d]), inv);
-                    else if (!all_new) y[e] = grew && tt < t0 ? code_value<Code>(z[e], again) : z[e];
+                    y[e] = code_value<Code>(load_acc(r[4 * q + e]), inv);
+                    if (!all_new && !(tt >= t0 && tt < t1)) y[e] = grew && tt < t0 ? code_value<Code>(z[e], again) : z[e];
                 }
                 const uint32_t made = Code::encode(y);
                 // codes that stay keep their bits (a NaN's payload, int8's -128)
@@ -182,20 +190,27 @@ __global__ __launch_bounds__(THREADS) void kvcache_read_kernel(const RowsArgs a)
             }
         }
     } else {
+        // as many dimensions a lane as make a dword of a row
+        constexpr int N = 4 / (int)sizeof(T);
         const int c0 = t0 / 16, c1 = (t1 + 15) / 16;
-        for (int i = threadIdx.x; i < (c1 - c0) * D; i += THREADS) {
-            const int c = c0 + i / D, d = i % D, t = c * 16;
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if (page >= 0) w = *reinterpret_cast<const u32x4 *>(codes + d * P + t);
+        for (int i = threadIdx.x; i < (c1 - c0) * (D / N); i += THREADS) {
+            const int c = c0 + i / (D / N), d = i % (D / N) * N, t = c * 16;
+            float y[N][16];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float y[4];
-                Code::decode(w[q], y);
+            for (int k = 0; k < N; ++k) {
+                u32x4 w = {0u, 0u, 0u, 0u};
+                if (page >= 0) w = *reinterpret_cast<const u32x4 *>(codes + (d + k) * P + t);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int tt = t + 4 * q + e;
-                    if (tt >= t0 && tt < t1) x[(tt - t0) * pitch + d] = store_acc<T>(y[e] * scale);
-                }
+                for (int q = 0; q < 4; ++q) Code::decode(w[q], y[k] + 4 * q);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float z[N];
+                vec_t<T, N> r;
+#pragma unroll
+                for (int k = 0; k < N; ++k) z[k] = y[k][e] * scale;
+                store_acc_vec<T, N>(r, z);
+                if (t + e >= t0 && t + e < t1) *reinterpret_cast<vec_t<T, N> *>(x + (t + e - t0) * pitch + d) = r;
             }
         }
     }

@@ -12,6 +12,7 @@
 // lanes (`lg`) holds the head: sums are shuffles inside the group, and the other value of a pair is in the same lane
 // (neighbouring pairs) or comes from lane +- R/2/V by one shuffle per value.  A lane group keeps its row while it walks
 // over that row's heads, so the cosines and sines are loaded once per row and group, not once per head.
+#include <algorithm>
 #include "matmul_common.hpp"
 
 using namespace dxh;
@@ -32,22 +33,29 @@ struct Args {
     const float *cos, *sin;
     const void *positions;
     int64_t rows, table_rows;
-    int dim, rd, pos_i64;
+    int dim, rd, pos_i64, nt;  // nt: the results are too many bytes to be found in the last-level cache by whoever reads them
     float eps;
     float *partial;  // backward: [part][workgroup][dim]
 };
 
 // V consecutive values of a head as fp32
 template <typename T> constexpr int kV = kVecBytes / (int)sizeof(T);
-template <typename T> __device__ __forceinline__ void load_vec(const T *p, float (&x)[kV<T>]) {
-    const vec_t<T, kV<T>> r = *reinterpret_cast<const vec_t<T, kV<T>> *>(p);
+template <typename T> using Piece = vec_t<T, kV<T>>;
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *p, bool live) {
+    Piece<T> r = {};
+    if (live) r = *reinterpret_cast<const Piece<T> *>(p);
+    return r;
+}
+template <typename T> __device__ __forceinline__ void unpack(const Piece<T> &r, float (&x)[kV<T>]) {
 #pragma unroll
     for (int e = 0; e < kV<T>; ++e) x[e] = load_acc(r.v[e]);
 }
-template <typename T> __device__ __forceinline__ void store_vec(T *p, const float (&x)[kV<T>]) {
-    vec_t<T, kV<T>> r;
+template <typename T> __device__ __forceinline__ void load_vec(const T *p, float (&x)[kV<T>]) { unpack<T>(*reinterpret_cast<const Piece<T> *>(p), x); }
+template <typename T> __device__ __forceinline__ void store_vec(T *p, const float (&x)[kV<T>], int nt) {
+    Piece<T> r;
     store_acc_vec<T, kV<T>>(r, x);
-    *reinterpret_cast<vec_t<T, kV<T>> *>(p) = r;
+    if (nt) st_mode<1>(reinterpret_cast<Piece<T> *>(p), r);
+    else *reinterpret_cast<Piece<T> *>(p) = r;
 }
 template <typename T> __device__ __forceinline__ void load_weight(const Part &p, int d, float (&w)[kV<T>]) {
 #pragma unroll
@@ -151,11 +159,12 @@ __global__ __launch_bounds__(kBlock) void normrope_kernel(const Args a) {
         if (row >= a.rows) continue;  // whole lane groups leave together
         float c[V], s[V];
         load_angles<T, MODE>(a, row, d, live, c, s);
+        const T *src = (const T *)p.x + row * p.x_row + d;
+        Piece<T> next = load_piece<T>(src + sub * p.x_head, live && sub < p.heads);
         for (int h = sub; h < p.heads; h += p.groups) {
             float x[V], y[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = 0.f;
-            if (live) load_vec<T>((const T *)p.x + row * p.x_row + h * p.x_head + d, x);
+            unpack<T>(next, x);
+            next = load_piece<T>(src + (h + p.groups) * p.x_head, live && h + p.groups < p.heads);  // comes while this head is worked on
             if (p.norm) {
                 float sq = 0.f;
 #pragma unroll
@@ -165,7 +174,7 @@ __global__ __launch_bounds__(kBlock) void normrope_kernel(const Args a) {
                 for (int e = 0; e < V; ++e) x[e] *= r * w[e];
             }
             rotate<T, MODE, LG>(a, d, x, c, s, false, y);
-            if (live) store_vec<T>((T *)p.out + row * p.o_row + h * p.o_head + d, y);
+            if (live) store_vec<T>((T *)p.out + row * p.o_row + h * p.o_head + d, y, a.nt);
         }
     }
 }
@@ -191,12 +200,15 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
         if (row >= a.rows) continue;
         float c[V], s[V];
         load_angles<T, MODE>(a, row, d, live, c, s);
+        const T *src = (const T *)p.x + row * p.x_row + d, *dsrc = (const T *)p.y_in + row * p.y_row + d;
+        Piece<T> next_x = load_piece<T>(src + sub * p.x_head, live && p.norm && sub < p.heads), next_dy = load_piece<T>(dsrc + sub * p.y_head, live && sub < p.heads);
         for (int h = sub; h < p.heads; h += p.groups) {
             float x[V], dy[V], g[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) { x[e] = 0.f; dy[e] = 0.f; }
-            if (live) load_vec<T>((const T *)p.y_in + row * p.y_row + h * p.y_head + d, dy);
-            if (live && p.norm) load_vec<T>((const T *)p.x + row * p.x_row + h * p.x_head + d, x);
+            unpack<T>(next_x, x);
+            unpack<T>(next_dy, dy);
+            const int h1 = h + p.groups;
+            next_x = load_piece<T>(src + h1 * p.x_head, live && p.norm && h1 < p.heads);
+            next_dy = load_piece<T>(dsrc + h1 * p.y_head, live && h1 < p.heads);
             rotate<T, MODE, LG>(a, d, dy, c, s, true, g);
             if (p.norm) {
                 float sq = 0.f, hx = 0.f;
@@ -213,7 +225,7 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
                     g[e] = r * __builtin_fmaf(-x[e], k, g[e] * w[e]);
                 }
             }
-            if (live) store_vec<T>((T *)p.out + row * p.o_row + h * p.o_head + d, g);
+            if (live) store_vec<T>((T *)p.out + row * p.o_row + h * p.o_head + d, g, a.nt);
         }
     }
     if (!p.dw) return;  // the same for the whole workgroup
@@ -227,21 +239,25 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
     }
 }
 
-// dw[i] = sum over n workgroups of partial[i]: 16 columns a workgroup, 16 lanes a column, each a run of workgroups
-__global__ __launch_bounds__(kBlock) void sum_partials_kernel(const Args a, int n) {
-    __shared__ float meet[kBlock];
+// dw[i] = sum over n workgroups of partial[i]: 16 columns a workgroup, 64 lanes a column, each every 64th workgroup
+constexpr int kSumLanes = 64;
+__global__ __launch_bounds__(16 * kSumLanes) void sum_partials_kernel(const Args a, int n) {
+    __shared__ float meet[16 * kSumLanes];
     const Part &p = a.part[blockIdx.y];
     if (!p.dw) return;
     const int col = blockIdx.x * 16 + threadIdx.x % 16, lane = threadIdx.x / 16;
     const float *src = a.partial + (int64_t)blockIdx.y * n * a.dim + col;
     float t = 0.f;
-    for (int i = lane; i < n; i += 16) t += src[(int64_t)i * a.dim];  // dim is a multiple of 16: every column exists
+#pragma unroll 8
+    for (int i = lane; i < n; i += kSumLanes) t += src[(int64_t)i * a.dim];  // dim is a multiple of 16: every column exists
     meet[threadIdx.x] = t;
     __syncthreads();
-    if (lane == 0) {
-        for (int k = 1; k < 16; ++k) t += meet[k * 16 + threadIdx.x];
-        p.dw[col] = t;
+#pragma unroll
+    for (int half = kSumLanes / 2; half > 0; half /= 2) {
+        if (lane < half) meet[threadIdx.x] += meet[threadIdx.x + half * 16];
+        __syncthreads();
     }
+    if (lane == 0) p.dw[col] = meet[threadIdx.x];
 }
 
 constexpr int kBackwardMaxGroups = 512;  // most workgroups along the rows: bounds the workspace, 2 a CU
@@ -275,9 +291,11 @@ int check(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, i
     const int es = dtype_size(dtype), v = kVecBytes / es;
     int lg = 4;
     while (lg * v < dim) lg *= 2;
+    int64_t heads = 0;
     for (int i = 0; i < nparts; ++i) {
         const dxh_normrope_part &s = parts[i];
         Part &p = a.part[i];
+        heads += s.heads > 0 ? s.heads : 0;
         if (s.heads < 0 || (s.norm != 0 && s.norm != 1)) return DXH_ERR_ARG;
         if (s.weight && s.weight_dtype != dtype && s.weight_dtype != DXH_F32) return DXH_ERR_DTYPE;
         const dxh_heads &out = back ? s.dx : s.y;
@@ -300,6 +318,7 @@ int check(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, i
         while (g < most && g * (rows < 4 * kCUs ? 1 : 4) < s.heads) g *= 2;
         p.groups = g;
     }
+    a.nt = use_nt_store((size_t)rows * heads * dim * es);
     return DXH_OK;
 }
 int slots_of(const Args &a, int nparts, int lg) {  // fewest rows that a workgroup of any part takes at once
@@ -395,7 +414,7 @@ int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int nparts,
     const int lg = lanes_of(dtype, dim), groups = backward_groups(a, nparts, lg);
     rc = launch_dtype(dtype, a, nparts, rot, true, lg, (unsigned)groups, st);
     if (rc != DXH_OK || !need) return rc;
-    sum_partials_kernel<<<dim3(dim / 16, nparts), kBlock, 0, st>>>(a, groups);
+    sum_partials_kernel<<<dim3(dim / 16, nparts), 16 * kSumLanes, 0, st>>>(a, groups);
     return launch_status();
 }
 

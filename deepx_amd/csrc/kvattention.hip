@@ -798,6 +798,7 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     if ((rc = kv_heads_check(q, es, used)) != DXH_OK || (rc = kv_heads_check(out, es, used)) != DXH_OK) return rc;
     if (!aligned(lse, 4)) return DXH_ERR_ALIGN;
     if (!used) return DXH_OK;
+    if (q->data == out->data) return DXH_ERR_ARG;  // a row's queries are read by several workgroups
     const size_t need = part_bytes(a.kv, q_heads, a.splits);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return DXH_ERR_WORKSPACE;
     a.q = (const char *)q->data; a.q_row = q->row_stride; a.q_head = q->head_stride;

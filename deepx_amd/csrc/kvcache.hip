@@ -245,6 +245,7 @@ int rows_call(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, const
         a.head_stride[i] = h->head_stride;
     }
     if (!used) return DXH_OK;
+    if (!write && a.data[0] == a.data[1]) return DXH_ERR_ARG;  // two results in one place
     // n rows that start anywhere in a page touch at most this many
     a.slots = (int)(((int64_t)a.kv.max_rows + a.kv.page_size - 2) / a.kv.page_size) + 1;
     hipStream_t st = as_stream(stream);

@@ -318,6 +318,14 @@ int check(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, i
         while (g < most && g * (rows < 4 * kCUs ? 1 : 4) < s.heads) g *= 2;
         p.groups = g;
     }
+    // a result may lie where its own inputs do, and nowhere else among what the launch touches
+    for (int i = 0; i < nparts; ++i)
+        for (int j = 0; j < nparts; ++j) {
+            const Part &p = a.part[i], &q = a.part[j];
+            if (i == j || rows == 0 || !p.heads || !q.heads) continue;
+            if (p.out == q.out || p.out == q.x || (back && p.out == q.y_in)) return DXH_ERR_ARG;
+            if (p.dw && p.dw == q.dw) return DXH_ERR_ARG;
+        }
     a.nt = use_nt_store((size_t)rows * heads * dim * es);
     return DXH_OK;
 }

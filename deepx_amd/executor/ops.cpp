@@ -84,10 +84,11 @@ void reg(TfFactory &f, const char *name, const char *author, const char *tftype,
     if (op == "sum") { tf->chain_code = DXH_CHAIN_ROWSUM; tf->chain_kind = 8; }
     if (op == "reducemax") { tf->chain_code = DXH_CHAIN_ROWMAX; tf->chain_kind = 8; }
     if (op == "reducemin") { tf->chain_code = DXH_CHAIN_ROWMIN; tf->chain_kind = 8; }
-    tf->graph_safe = kind == "elementwise" || kind == "reduce" || kind == "changeshape" || op == "matmul" ||
+    tf->graph_safe = kind == "elementwise" || kind == "reduce" || kind == "changeshape" || kind == "attention" || op == "matmul" ||
                      op == "constant" || op == "arange";
     if (op == "reshape") tf->graph_safe = false;  // rewrites the tensor's shape on the host
-    tf->overwrites_results = tf->graph_safe || op == "uniform" || op == "normal" || op == "copytensor" || op == "loadtensordata";
+    // the lines over a cache leave parts of their results as they were: older tokens, rows of no sequence
+    tf->overwrites_results = (tf->graph_safe && op.rfind("kvcache", 0) != 0) || op == "uniform" || op == "normal" || op == "copytensor" || op == "loadtensordata";
     f.add_tf(tf);
 }
 
@@ -264,6 +265,107 @@ RunFn reduce(ReduceFn f, const char *op) {  // (A, vector dims, bool keepdims) -
         return hip_result(f(A->dtype(), A->data, A->shape.shape.data(), A->shape.dim(), dims.data(), (int)dims.size(), B->data, ws,
                             need ? mem.workspace_bytes() : 0, mem.stream), op, error);
     };
+}
+
+// ---- attention lines ---------------------------------------------------------------------------
+// a list of tensors "[a b c]" (or one name)
+std::vector<std::shared_ptr<Tensor>> tensors_of_list(const Param &p, Mem &mem) {
+    std::vector<std::shared_ptr<Tensor>> ts;
+    for (auto &n : words_of(p)) ts.push_back(mem.gettensor(n));
+    return ts;
+}
+[[noreturn]] void bad_shape(const std::string &what, const Tensor &t) { throw std::invalid_argument(what + ", got " + precision_str(t.shape.dtype) + dims_str(t.shape.shape)); }
+const Tensor &need(const Tensor &t, Precision p, int dim, const char *what) {
+    if (t.shape.dtype != p || t.shape.dim() != dim) bad_shape(std::string(what) + " must be " + precision_str(p) + " with " + std::to_string(dim) + " dims", t);
+    return t;
+}
+// the [rows, heads, dim] view of a contiguous tensor
+dxh_heads heads_view(const Tensor &t) {
+    if (t.shape.dim() != 3) bad_shape("rows must be a [rows, heads, dim] tensor", t);
+    return {t.data, (int64_t)t.shape.at(1) * t.shape.at(2), t.shape.at(2)};
+}
+dxh_rotary rotary_of(const Param &cos, const Param &sin, const Param &positions, bool interleaved, int64_t rows, Mem &mem) {
+    auto C = tensor_of(cos, mem), S = tensor_of(sin, mem), P = tensor_of(positions, mem);
+    need(*C, Precision::Float32, 2, "cos");
+    need(*S, Precision::Float32, 2, "sin");
+    if (C->shape.shape != S->shape.shape) bad_shape("cos and sin must have one shape", *S);
+    if (P->shape.dtype != Precision::Int32 && P->shape.dtype != Precision::Int64) throw std::invalid_argument("positions only support int32 or int64");
+    if (P->shape.size != rows) bad_shape("positions must hold one entry a row", *P);
+    return {(const float *)C->data, (const float *)S->data, P->data, C->shape.at(0), 2 * C->shape.at(1), interleaved ? 1 : 0, P->dtype()};
+}
+// normrope / rope and the gradients: tensors of the same rows and head size, each with its weight (none for rope)
+struct NormropeCall {
+    std::vector<dxh_normrope_part> parts;
+    int dtype = 0, dim = 0;
+    int64_t rows = 0;
+    NormropeCall(const Param &xs, const Param &ys, const Param *weights, const Param *dxs, const Param *dws, Mem &mem) {
+        auto x = tensors_of_list(xs, mem), y = tensors_of_list(ys, mem);
+        std::vector<std::shared_ptr<Tensor>> w, g, dw;
+        if (weights) w = tensors_of_list(*weights, mem);
+        if (dxs) g = tensors_of_list(*dxs, mem);
+        if (dws) dw = tensors_of_list(*dws, mem);
+        if (x.empty() || x.size() > DXH_NORMROPE_MAX_PARTS) throw std::invalid_argument("one to " + std::to_string(DXH_NORMROPE_MAX_PARTS) + " tensors at a time");
+        if (y.size() != x.size() || (weights && w.size() != x.size()) || (dxs && g.size() != x.size()) || (dws && dw.size() != x.size()))
+            throw std::invalid_argument("as many of each list of tensors as there are inputs");
+        for (size_t i = 0; i < x.size(); ++i) {
+            dxh_normrope_part p{};
+            p.x = heads_view(*x[i]);
+            if (i == 0) { dtype = x[0]->dtype(); rows = x[0]->shape.at(0); dim = x[0]->shape.at(2); }
+            if (x[i]->dtype() != dtype || x[i]->shape.at(0) != rows || x[i]->shape.at(2) != dim) bad_shape("tensors must agree in dtype, rows and head size", *x[i]);
+            for (const auto &like : {y[i], dxs ? g[i] : y[i]})
+                if (like->dtype() != dtype || like->shape.shape != x[i]->shape.shape) bad_shape("tensors of one head group must have one dtype and shape " + dims_str(x[i]->shape.shape), *like);
+            p.y = heads_view(*y[i]);
+            if (dxs) p.dx = heads_view(*g[i]);
+            if (weights) {
+                if (w[i]->shape.size != dim) bad_shape("a weight must hold one value for each of the head's " + std::to_string(dim), *w[i]);
+                p.weight = w[i]->data;
+                p.weight_dtype = w[i]->dtype();
+                p.norm = 1;
+            }
+            if (dws) {
+                if (dw[i]->shape.dtype != Precision::Float32 || dw[i]->shape.size != dim) bad_shape("a weight's gradient must be float32 with one value for each of the head's " + std::to_string(dim), *dw[i]);
+                p.dweight = (float *)dw[i]->data;
+            }
+            p.heads = x[i]->shape.at(1);
+            parts.push_back(p);
+        }
+    }
+};
+// the cache "[k v k_scale v_scale]", whose codes travel in int8 tensors whatever they stand for
+dxh_kvcache cache_of(const Param &list, const Param &table, const Param &code, Mem &mem) {
+    auto ts = tensors_of_list(list, mem);
+    if (ts.size() != 4) throw std::invalid_argument("a cache is four tensors: keys, values, key scales, value scales");
+    auto T = tensor_of(table, mem);
+    need(*ts[0], Precision::Int8, 4, "cached keys");
+    need(*ts[1], Precision::Int8, 4, "cached values");
+    need(*ts[2], Precision::Float32, 2, "key scales");
+    need(*ts[3], Precision::Float32, 2, "value scales");
+    need(*T, Precision::Int32, 2, "the page table");
+    const std::vector<int> &k = ts[0]->shape.shape;  // [pages, heads, page, dim]
+    if (ts[1]->shape.shape != std::vector<int>{k[0], k[1], k[3], k[2]}) bad_shape("cached values must be " + dims_str({k[0], k[1], k[3], k[2]}), *ts[1]);
+    for (int i : {2, 3}) if (ts[i]->shape.shape != std::vector<int>{k[0], k[1]}) bad_shape("scales must be " + dims_str({k[0], k[1]}), *ts[i]);
+    dxh_kvcache c{};
+    c.k = ts[0]->data; c.v = ts[1]->data;
+    c.k_scale = (float *)ts[2]->data; c.v_scale = (float *)ts[3]->data;
+    c.page_table = (const int32_t *)T->data;
+    c.num_pages = k[0]; c.heads = k[1]; c.page_size = k[2]; c.dim = k[3];
+    c.pages_per_seq = T->shape.at(1);
+    if (code.textvalue == "int8") c.code = DXH_I8;
+    else if (code.textvalue == "float8e4m3") c.code = DXH_F8E4M3;
+    else throw std::invalid_argument("code must be int8 or float8e4m3, got " + code.textvalue);
+    return c;
+}
+dxh_kvrows kvrows_of(const Param &offsets, const Param &lengths, const Param &table, const Param &max_rows, int64_t rows, Mem &mem) {
+    auto O = tensor_of(offsets, mem), L = tensor_of(lengths, mem), T = tensor_of(table, mem);
+    need(*O, Precision::Int32, 1, "offsets");
+    need(*L, Precision::Int32, 1, "lengths");
+    if (O->shape.size != L->shape.size + 1) bad_shape("offsets must hold one entry more than there are sequences", *O);
+    if (T->shape.at(0) != L->shape.size) bad_shape("the page table must have a row for each sequence", *T);
+    return {(const int32_t *)O->data, (const int32_t *)L->data, rows, (int32_t)L->shape.size, int_of(max_rows, mem)};
+}
+void rows_match(const dxh_kvcache &c, const Tensor &t, bool key_heads) {
+    if (t.shape.at(2) != c.dim || (key_heads && t.shape.at(1) != c.heads))
+        bad_shape("rows must have the cache's " + (key_heads ? std::to_string(c.heads) + " heads and " : std::string()) + "head size " + std::to_string(c.dim), t);
 }
 
 // "T1 = zeros(shape)", as op-cuda's newtensor documents itself (its storage is whatever cudaMalloc returns).  The fill is
@@ -561,6 +663,87 @@ int register_all(TfFactory &f) {
     };
     for (const char *author : {"cublas", "cblas", "miaobyte"})
         reg(f, "matmul", author, "matmul", "T3=T1 @ T2", {T_ANY ":A", T_ANY ":B"}, {T_ANY ":C"}, matmul);
+
+    // ---- attention: no counterpart among the reference's registrations, whose front spells these steps as sin / cos / mul / add /
+    // concat and matmul + softmax + matmul lines (front/py/deepx/nn/modules/transformer/rotary_embedding.py:50-71, attention.py:15-32)
+#define T_LIST "listtensor<any>"
+    reg(f, "rope", "miaobyte", "attention", "Y=rotate(X,cos[pos],sin[pos])", {T_LIST ":X", "tensor<float32>:cos", "tensor<float32>:sin", "tensor<int64|int32>:positions", "var<bool>:interleaved"}, {T_LIST ":Y"},
+        [](const TF &c, Mem &mem, std::string &error) {
+            NormropeCall n(c.args[0], c.returns[0], nullptr, nullptr, nullptr, mem);
+            const dxh_rotary r = rotary_of(c.args[1], c.args[2], c.args[3], bool_of(c.args[4]), n.rows, mem);
+            return hip_result(dxh_normrope(n.dtype, n.parts.data(), (int)n.parts.size(), n.rows, n.dim, 0.f, &r, mem.stream), "rope", error);
+        });
+    reg(f, "normrope", "miaobyte", "attention", "Y=rotate(W*X/sqrt(mean(X^2)+eps),cos[pos],sin[pos])",
+        {T_LIST ":X", T_LIST ":W", "tensor<float32>:cos", "tensor<float32>:sin", "tensor<int64|int32>:positions", "var<any>:eps", "var<bool>:interleaved"}, {T_LIST ":Y"},
+        [](const TF &c, Mem &mem, std::string &error) {
+            NormropeCall n(c.args[0], c.returns[0], &c.args[1], nullptr, nullptr, mem);
+            const dxh_rotary r = rotary_of(c.args[2], c.args[3], c.args[4], bool_of(c.args[6]), n.rows, mem);
+            return hip_result(dxh_normrope(n.dtype, n.parts.data(), (int)n.parts.size(), n.rows, n.dim, float_of(c.args[5], mem), &r, mem.stream), "normrope", error);
+        });
+    reg(f, "normropebackward", "miaobyte", "attention", "dX,dW=gradients(normrope,dY)",
+        {T_LIST ":X", T_LIST ":dY", T_LIST ":W", "tensor<float32>:cos", "tensor<float32>:sin", "tensor<int64|int32>:positions", "var<any>:eps", "var<bool>:interleaved"}, {T_LIST ":dX", T_LIST ":dW"},
+        [](const TF &c, Mem &mem, std::string &error) {
+            NormropeCall n(c.args[0], c.args[1], &c.args[2], &c.returns[0], &c.returns[1], mem);
+            const dxh_rotary r = rotary_of(c.args[3], c.args[4], c.args[5], bool_of(c.args[7]), n.rows, mem);
+            size_t bytes = 0;
+            const int rc = dxh_normrope_backward_workspace_bytes(n.dtype, n.parts.data(), (int)n.parts.size(), n.rows, n.dim, &bytes);
+            if (rc != DXH_OK) return hip_result(rc, "normropebackward", error);
+            void *ws = bytes ? mem.workspace(bytes) : nullptr;
+            return hip_result(dxh_normrope_backward(n.dtype, n.parts.data(), (int)n.parts.size(), n.rows, n.dim, float_of(c.args[6], mem), &r, ws, bytes ? mem.workspace_bytes() : 0, mem.stream),
+                              "normropebackward", error);
+        });
+    reg(f, "kvcachewrite", "miaobyte", "attention", "cache[pages[pos]]=quantise(K,V)",
+        {T_ANY ":K", T_ANY ":V", "tensor<int32>:offsets", "tensor<int32>:lengths", "tensor<int32>:pages", "var<int32>:max_rows", "var<string>:code"}, {T_LIST ":cache"},
+        [](const TF &c, Mem &mem, std::string &error) {
+            auto K = tensor_of(c.args[0], mem), V = tensor_of(c.args[1], mem);
+            if (!same_dtype({K.get(), V.get()}, error)) return 1;
+            const dxh_heads k = heads_view(*K), v = heads_view(*V);
+            if (K->shape.shape != V->shape.shape) return fail(error, "shape mismatch: " + dims_str(K->shape.shape) + " vs " + dims_str(V->shape.shape));
+            const dxh_kvcache cache = cache_of(c.returns[0], c.args[4], c.args[6], mem);
+            rows_match(cache, *K, true);
+            const dxh_kvrows rows = kvrows_of(c.args[2], c.args[3], c.args[4], c.args[5], K->shape.at(0), mem);
+            return hip_result(dxh_kvcache_write(&cache, &rows, K->dtype(), &k, &v, mem.stream), "kvcachewrite", error);
+        });
+    reg(f, "kvcacheread", "miaobyte", "attention", "K,V=cache[pages[pos]]*scale",
+        {T_LIST ":cache", "tensor<int32>:offsets", "tensor<int32>:lengths", "tensor<int32>:pages", "var<int32>:max_rows", "var<string>:code"}, {T_ANY ":K", T_ANY ":V"},
+        [](const TF &c, Mem &mem, std::string &error) {
+            auto K = tensor_of(c.returns[0], mem), V = tensor_of(c.returns[1], mem);
+            if (!same_dtype({K.get(), V.get()}, error)) return 1;
+            const dxh_heads k = heads_view(*K), v = heads_view(*V);
+            if (K->shape.shape != V->shape.shape) return fail(error, "shape mismatch: " + dims_str(K->shape.shape) + " vs " + dims_str(V->shape.shape));
+            const dxh_kvcache cache = cache_of(c.args[0], c.args[3], c.args[5], mem);
+            rows_match(cache, *K, true);
+            const dxh_kvrows rows = kvrows_of(c.args[1], c.args[2], c.args[3], c.args[4], K->shape.at(0), mem);
+            return hip_result(dxh_kvcache_read(&cache, &rows, K->dtype(), &k, &v, mem.stream), "kvcacheread", error);
+        });
+    auto attention = [](const TF &c, Mem &mem, std::string &error) {
+        auto Q = tensor_of(c.args[0], mem), O = tensor_of(c.returns[0], mem);
+        if (!same_dtype({Q.get(), O.get()}, error)) return 1;
+        const dxh_heads q = heads_view(*Q), o = heads_view(*O);
+        if (Q->shape.shape != O->shape.shape) return fail(error, "shape mismatch: " + dims_str(Q->shape.shape) + " vs " + dims_str(O->shape.shape));
+        if (Q->data == O->data) return fail(error, "kvcacheattention cannot run in place");
+        float *lse = nullptr;
+        std::shared_ptr<Tensor> L;
+        if (c.returns.size() > 1) {
+            L = tensor_of(c.returns[1], mem);
+            if (L->shape.dtype != Precision::Float32 || L->shape.size != (int64_t)Q->shape.at(0) * Q->shape.at(1)) bad_shape("lse must be float32 with one value for each row and query head", *L);
+            lse = (float *)L->data;
+        }
+        const dxh_kvcache cache = cache_of(c.args[1], c.args[4], c.args[9], mem);
+        rows_match(cache, *Q, false);
+        const dxh_kvrows rows = kvrows_of(c.args[2], c.args[3], c.args[4], c.args[5], Q->shape.at(0), mem);
+        size_t bytes = 0;
+        const int rc = dxh_kvcache_attention_workspace_bytes(&cache, &rows, Q->dtype(), Q->shape.at(1), &bytes);
+        if (rc != DXH_OK) return hip_result(rc, "kvcacheattention", error);
+        void *ws = bytes ? mem.workspace(bytes) : nullptr;
+        return hip_result(dxh_kvcache_attention(&cache, &rows, Q->dtype(), Q->shape.at(1), &q, &o, lse, float_of(c.args[6], mem), bool_of(c.args[7]) ? 1 : 0, scalar_of(c.args[8], mem).i, ws,
+                                                bytes ? mem.workspace_bytes() : 0, mem.stream), "kvcacheattention", error);
+    };
+#define ATTENTION_ARGS {T_ANY ":Q", T_LIST ":cache", "tensor<int32>:offsets", "tensor<int32>:lengths", "tensor<int32>:pages", "var<int32>:max_rows", "var<any>:scale", "var<bool>:causal", "var<any>:window", "var<string>:code"}
+    reg(f, "kvcacheattention", "miaobyte", "attention", "O=softmax(scale*Q@K)@V over cache[pages]", ATTENTION_ARGS, {T_ANY ":O"}, attention);
+    reg(f, "kvcacheattention", "miaobyte", "attention", "O,lse=softmax(scale*Q@K)@V over cache[pages]", ATTENTION_ARGS, {T_ANY ":O", "tensor<float32>:lse"}, attention);
+#undef ATTENTION_ARGS
+#undef T_LIST
 #undef T_ANY
     return 0;
 }

@@ -50,6 +50,16 @@ def test_normrope():
         assert fwd(norm_part(x=bad), rows=1) == ALIGN and fwd(norm_part(y=bad), rows=1) == ALIGN
 
 
+def test_results_that_would_overwrite_other_inputs():
+    """two parts whose results meet, or meet the other part's input, are refused (a result in its own input's place is not)"""
+    L = dx.load()
+    two = lambda x0, y0, x1, y1: (dx.NormropePart * 2)(norm_part(x=heads(x0), y=heads(y0)), norm_part(x=heads(x1), y=heads(y1)))  # noqa: E731
+    for ptrs in ((4096, 8192, 16384, 8192), (4096, 16384, 16384, 4096), (4096, 8192, 8192, 16384)):
+        assert L.dxh_normrope(dx.BF16, two(*ptrs), 2, 1, 64, 1e-6, None, None) == ARG, ptrs
+    assert L.dxh_kvcache_read(cache(), kvrows(rows=1), dx.BF16, heads(), heads(), None) == ARG
+    assert L.dxh_kvcache_attention(cache(), kvrows(rows=1), dx.BF16, 14, heads(), heads(), None, 0.125, 1, 0, None, 0, None) == ARG
+
+
 def test_normrope_backward():
     L = dx.load()
     parts = (dx.NormropePart * 1)(norm_part())
@@ -90,7 +100,7 @@ BAD_ROWS = [(dict(batch=-1), ARG), (dict(rows=-1), ARG), (dict(max_rows=-1), ARG
 def test_kvcache_write_and_read():
     L = dx.load()
     for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
-        call = lambda c=None, r=None, dtype=dx.BF16, k=None, v=None: fn(c or cache(), r or kvrows(), dtype, k or heads(), v or heads(), None)  # noqa: E731, B023
+        call = lambda c=None, r=None, dtype=dx.BF16, k=None, v=None: fn(c or cache(), r or kvrows(), dtype, k or heads(), v or heads(16384), None)  # noqa: E731, B023
         assert call() == OK and call(cache(code=dx.F8E4M3)) == OK and call(cache(page_table=None, num_pages=32)) == OK
         for kw, rc in BAD_CACHE:
             assert call(cache(**kw)) == rc, kw

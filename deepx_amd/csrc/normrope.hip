@@ -9,9 +9,11 @@
 //
 // Everything between the load and the store is fp32; a result is rounded once.  The kernels are bound by memory: a head
 // is read once and written once, so a lane keeps a 16-byte piece of a head in registers and a power-of-two group of
-// lanes (`lg`) holds the head: sums are shuffles inside the group, and the other value of a pair is in the same lane
-// (neighbouring pairs) or comes from lane +- R/2/V by one shuffle per value.  A lane group keeps its row while it walks
-// over that row's heads, so the cosines and sines are loaded once per row and group, not once per head.
+// lanes (`lg`) holds the head: sums are cross-lane adds inside the group, and the other value of a pair is in the same lane
+// (neighbouring pairs) or comes from lane +- R/2/V.  A lane group keeps its row while it walks over that row's heads, so the
+// cosines and sines are loaded once per row and group, not once per head.  Measured: 16384 rows of 32 + 8 heads of 128 in bf16
+// 62.9 us (5.5 TB/s); backward of 8192 such rows 49.5 us (5.2 TB/s).  Several heads' loads at once cost more in occupancy than
+// they hide (two: 64.9, four: 87 us).
 #include <algorithm>
 #include "matmul_common.hpp"
 
@@ -41,9 +43,11 @@ struct Args {
 // V consecutive values of a head as fp32
 template <typename T> constexpr int kV = kVecBytes / (int)sizeof(T);
 template <typename T> using Piece = vec_t<T, kV<T>>;
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *p, bool live) {
+// A launch that stores more than the last-level cache is good for (use_nt_store) reads and writes past it: 16384 rows of 40
+// heads of 128 in bf16, plain 71.5 us; stores nt 71.5; loads nt too 63.3; stores nt at agent scope 62.9.
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *p, bool live, int nt) {
     Piece<T> r = {};
-    if (live) r = *reinterpret_cast<const Piece<T> *>(p);
+    if (live) r = nt ? ld_nt(reinterpret_cast<const Piece<T> *>(p)) : *reinterpret_cast<const Piece<T> *>(p);
     return r;
 }
 template <typename T> __device__ __forceinline__ void unpack(const Piece<T> &r, float (&x)[kV<T>]) {
@@ -54,7 +58,7 @@ template <typename T> __device__ __forceinline__ void load_vec(const T *p, float
 template <typename T> __device__ __forceinline__ void store_vec(T *p, const float (&x)[kV<T>], int nt) {
     Piece<T> r;
     store_acc_vec<T, kV<T>>(r, x);
-    if (nt) st_mode<1>(reinterpret_cast<Piece<T> *>(p), r);
+    if (nt) st_mode<3>(reinterpret_cast<Piece<T> *>(p), r);
     else *reinterpret_cast<Piece<T> *>(p) = r;
 }
 template <typename T> __device__ __forceinline__ void load_weight(const Part &p, int d, float (&w)[kV<T>]) {
@@ -69,15 +73,35 @@ template <typename T> __device__ __forceinline__ void load_weight(const Part &p,
         load_vec<T>((const T *)p.w + d, w);
     }
 }
+// A value of another lane by the vector pipe's own cross-lane paths: no LDS access, which the shuffles of a head (a sum and one
+// value an element) would otherwise need about 12 of for 16 bytes.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return bits_to_float((uint32_t)__builtin_amdgcn_mov_dpp((int)float_to_bits(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kQuadReverse = 0x1b, kRowRor8 = 0x128, kRowMirror = 0x140, kHalfMirror = 0x141;
+// The sum over a group of LG lanes, in every lane.  Lanes of a quad, then of eight, then of sixteen agree after a step, so that
+// a mirror reaches the other half as well as an exclusive or would.
 template <int LG> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, LG);
+    v += dpp<kQuadXor1>(v);
+    v += dpp<kQuadXor2>(v);
+    if constexpr (LG >= 8) v += dpp<kHalfMirror>(v);
+    if constexpr (LG >= 16) v += dpp<kRowMirror>(v);
+    if constexpr (LG >= 32) v += __shfl_xor(v, 16);
+    if constexpr (LG >= 64) v += __shfl_xor(v, 32);
     return v;
+}
+// the value of lane ^ LG/2
+template <int LG> __device__ __forceinline__ float other_half(float v) {
+    if constexpr (LG == 4) return dpp<kQuadXor2>(v);
+    else if constexpr (LG == 8) return dpp<kQuadReverse>(dpp<kHalfMirror>(v));
+    else if constexpr (LG == 16) return dpp<kRowRor8>(v);
+    else return __shfl_xor(v, LG / 2);
 }
 
 // How the values of a pair meet: kNear pairs (2i, 2i + 1) share a lane; kFar pairs (i, i + R/2) with R/2 a multiple of V
-// are the same element of the lane R/2/V further; kAny is kFar with any even R: element by element through shuffles.
-enum { kNear = 0, kFar = 1, kAny = 2 };
+// are the same element of the lane R/2/V further, kHalf those of a head that is rotated whole and fills its lanes (the other
+// lane is lane ^ LG/2); kAny is kFar with any even R: element by element through shuffles.
+enum { kNear = 0, kFar = 1, kAny = 2, kHalf = 3 };
 
 // cosine and sine of every element of this lane's piece and the sign its partner's product gets; elements past R: c = 1, s = 0
 template <typename T, int MODE>
@@ -91,7 +115,7 @@ __device__ __forceinline__ void load_angles(const Args &a, int64_t row, int d, b
     p = p < 0 ? 0 : p >= a.table_rows ? a.table_rows - 1 : p;
     const int half = a.rd / 2;
     const float *ct = a.cos + p * half, *st = a.sin + p * half;
-    if constexpr (MODE == kFar) {  // whole 16-byte pieces of the table
+    if constexpr (MODE == kFar || MODE == kHalf) {  // whole 16-byte pieces of the table
         const bool hi = d >= half;
         const int i = hi ? d - half : d;
 #pragma unroll
@@ -118,6 +142,9 @@ __device__ __forceinline__ void rotate(const Args &a, int d, const float (&n)[kV
     if constexpr (MODE == kNear) {
 #pragma unroll
         for (int e = 0; e < V; ++e) y[e] = d + e < a.rd ? __builtin_fmaf(n[e], c[e], sign * (n[e ^ 1] * s[e])) : n[e];
+    } else if constexpr (MODE == kHalf) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = __builtin_fmaf(n[e], c[e], sign * (other_half<LG>(n[e]) * s[e]));
     } else if constexpr (MODE == kFar) {
         const int shift = half / V, me = d / V, from = d >= a.rd ? me : d >= half ? me - shift : me + shift;
 #pragma unroll
@@ -159,12 +186,9 @@ __global__ __launch_bounds__(kBlock) void normrope_kernel(const Args a) {
         if (row >= a.rows) continue;  // whole lane groups leave together
         float c[V], s[V];
         load_angles<T, MODE>(a, row, d, live, c, s);
-        const T *src = (const T *)p.x + row * p.x_row + d;
-        Piece<T> next = load_piece<T>(src + sub * p.x_head, live && sub < p.heads);
         for (int h = sub; h < p.heads; h += p.groups) {
             float x[V], y[V];
-            unpack<T>(next, x);
-            next = load_piece<T>(src + (h + p.groups) * p.x_head, live && h + p.groups < p.heads);  // comes while this head is worked on
+            unpack<T>(load_piece<T>((const T *)p.x + row * p.x_row + h * p.x_head + d, live, a.nt), x);
             if (p.norm) {
                 float sq = 0.f;
 #pragma unroll
@@ -200,15 +224,10 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
         if (row >= a.rows) continue;
         float c[V], s[V];
         load_angles<T, MODE>(a, row, d, live, c, s);
-        const T *src = (const T *)p.x + row * p.x_row + d, *dsrc = (const T *)p.y_in + row * p.y_row + d;
-        Piece<T> next_x = load_piece<T>(src + sub * p.x_head, live && p.norm && sub < p.heads), next_dy = load_piece<T>(dsrc + sub * p.y_head, live && sub < p.heads);
         for (int h = sub; h < p.heads; h += p.groups) {
             float x[V], dy[V], g[V];
-            unpack<T>(next_x, x);
-            unpack<T>(next_dy, dy);
-            const int h1 = h + p.groups;
-            next_x = load_piece<T>(src + h1 * p.x_head, live && p.norm && h1 < p.heads);
-            next_dy = load_piece<T>(dsrc + h1 * p.y_head, live && h1 < p.heads);
+            unpack<T>(load_piece<T>((const T *)p.y_in + row * p.y_row + h * p.y_head + d, live, a.nt), dy);
+            unpack<T>(load_piece<T>((const T *)p.x + row * p.x_row + h * p.x_head + d, live && p.norm, a.nt), x);
             rotate<T, MODE, LG>(a, d, dy, c, s, true, g);
             if (p.norm) {
                 float sq = 0.f, hx = 0.f;
@@ -218,11 +237,11 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
                     hx = __builtin_fmaf(g[e] * w[e], x[e], hx);
                 }
                 const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LG>(sq), inv_dim, a.eps));
-                const float k = group_sum<LG>(hx) * inv_dim * r * r;
+                const float q = group_sum<LG>(hx) * inv_dim * r * r;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     dw[e] = __builtin_fmaf(g[e], x[e] * r, dw[e]);
-                    g[e] = r * __builtin_fmaf(-x[e], k, g[e] * w[e]);
+                    g[e] = r * __builtin_fmaf(-x[e], q, g[e] * w[e]);
                 }
             }
             if (live) store_vec<T>((T *)p.out + row * p.o_row + h * p.o_head + d, g, a.nt);
@@ -260,7 +279,8 @@ __global__ __launch_bounds__(16 * kSumLanes) void sum_partials_kernel(const Args
     if (lane == 0) p.dw[col] = meet[threadIdx.x];
 }
 
-constexpr int kBackwardMaxGroups = 512;  // most workgroups along the rows: bounds the workspace, 2 a CU
+// most workgroups along the rows, which bounds the workspace: 8192 rows of 40 heads of 128 in bf16 take 72 us at 512, 58 at 1024, 61 at 2048 (with two heads at once)
+constexpr int kBackwardMaxGroups = 1024;
 
 bool heads_aligned(const dxh_heads &h, int es) {
     return aligned(h.data, kVecBytes) && (h.row_stride * es) % kVecBytes == 0 && (h.head_stride * es) % kVecBytes == 0;
@@ -347,13 +367,15 @@ int lanes_of(int dtype, int dim) {
 
 template <typename T, int LG> int launch(const Args &a, int nparts, const dxh_rotary *rot, bool back, unsigned groups, hipStream_t st) {
     const dim3 grid(groups, nparts);
-    const bool near = a.rd == 0 || (rot && rot->interleaved), far = !near && (a.rd / 2) % kV<T> == 0;
+    const bool near = a.rd == 0 || (rot && rot->interleaved), far = !near && (a.rd / 2) % kV<T> == 0, half = far && a.rd == a.dim && a.dim == LG * kV<T>;
     if (back) {
         if (near) normrope_backward_kernel<T, LG, kNear><<<grid, kBlock, 0, st>>>(a);
+        else if (half) normrope_backward_kernel<T, LG, kHalf><<<grid, kBlock, 0, st>>>(a);
         else if (far) normrope_backward_kernel<T, LG, kFar><<<grid, kBlock, 0, st>>>(a);
         else normrope_backward_kernel<T, LG, kAny><<<grid, kBlock, 0, st>>>(a);
     } else {
         if (near) normrope_kernel<T, LG, kNear><<<grid, kBlock, 0, st>>>(a);
+        else if (half) normrope_kernel<T, LG, kHalf><<<grid, kBlock, 0, st>>>(a);
         else if (far) normrope_kernel<T, LG, kFar><<<grid, kBlock, 0, st>>>(a);
         else normrope_kernel<T, LG, kAny><<<grid, kBlock, 0, st>>>(a);
     }

@@ -1,0 +1,779 @@
+// kvattention.hpp — attention of a ragged batch of rows over a paged cache in 8 bits.
+//
+// For one key head and one sequence the rows of all query heads that share it are one matrix Q [R, D], row r = i * G + g for
+// query row i and head g of the G that share the key head.  With codes K', V' and page scales k_s, v_s, in base 2:
+//     s_j = (Q K'^T)_j k_s(j) scale log2(e),     t_j = s_j + log2 v_s(j),     m = max t_j,     p_j = 2^(t_j - m),
+//     O   = sum p_j V'_j,     l = sum p_j / v_s(j),     out = O / l,     lse = ln 2 (m + log2 l).
+// Taking the value scale into the exponent keeps p in (0, 1] whatever the scales are, so that it can be rounded to f16 (held
+// 2^15 times as large: normal down to 2^-29 of the largest): 2^-11 of a term where bf16 would lose 2^-8, on the same matrix
+// instruction.  Codes are whole numbers below 2^8 or e4m3 values, exact in bf16 and in f16, and enter the products
+// exactly; scales are applied to scores in fp32.  Q is exact too: bf16 rows multiply bf16 keys, f16 rows f16 keys; f32 rows are split
+// into three bf16 parts (24 bits) and their p into two f16 parts, each part one more product.
+//
+// Everything is computed transposed, S^T = K' Q^T and O^T = V'^T P^T, so that the tokens of a score tile are rows of the
+// accumulator and a probability is already in the lane that feeds it to the second product: no exchange between lanes.
+// Which token a row of the first product is, is free; it is chosen so that a lane holds 16 consecutive tokens — of one page,
+// with one scale — and the matching piece of V' is 16 consecutive codes of one dimension in the cache's [dim][token] order.
+//
+// A page scale that is no finite number, or (where a mask cuts the tile) a NaN code among the values, must not reach rows
+// that do not see the token, and 0 * NaN is NaN: such values are taken as zeros and the token's score becomes NaN for the
+// rows that see it.
+#pragma once
+#include <algorithm>
+#include "kvcache.hpp"
+
+namespace dxh {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+struct AttArgs {
+    KvArgs kv;
+    const char *q;
+    char *out;
+    int64_t q_row, q_head, o_row, o_head;
+    float *lse, *part_o, *part_ml;  // partials: [slice][packed row][q head][dim] and [slice][packed row][q head][2]
+    float scale;                    // scale * log2(e)
+    int q_heads, group, causal, window, splits, row_tiles, tile_rows;
+};
+
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+constexpr float kNone = -__builtin_inff();
+constexpr float kLift = 15.f;        // probabilities are held 2^15 times as large: at most 2^15 in f16, whose largest number is 65504
+constexpr float kTinyScale = 0x1p-100f;  // value scales below it are multiplied into the codes: 1 / scale stays finite
+
+// ---- products ---------------------------------------------------------------------------------------------------------
+// Kind: the 16-bit type of keys and queries; QP, PP: parts that hold a query value, a probability
+template <typename T> struct RowType { using Kind = __bf16; static constexpr int QP = 1, PP = 1; };
+template <> struct RowType<f16_t> { using Kind = _Float16; static constexpr int QP = 1, PP = 1; };
+template <> struct RowType<float> { using Kind = __bf16; static constexpr int QP = 3, PP = 2; };
+
+template <typename Kind> __device__ __forceinline__ f32x4_t mma16(const u32x4 &a, const u32x4 &b, const f32x4_t &c) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename Kind> __device__ __forceinline__ f32x16 mma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename Kind> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same_v<Kind, __bf16>) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+// eight values -> N vectors of Kind whose sum they are, as far as N parts reach
+template <typename Kind, int N> __device__ __forceinline__ void split_parts(float (&x)[8], u32x4 (&p)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t w = pack2<Kind>(x[2 * e], x[2 * e + 1]);
+            p[k][e] = w;
+            if (k + 1 < N) {
+                if constexpr (std::is_same_v<Kind, __bf16>) {
+                    x[2 * e] -= bits_to_float(w << 16);
+                    x[2 * e + 1] -= bits_to_float(w & 0xffff0000u);
+                } else {
+                    const f16x2_t h = __builtin_bit_cast(f16x2_t, w);
+                    x[2 * e] -= (float)h[0];
+                    x[2 * e + 1] -= (float)h[1];
+                }
+            }
+        }
+}
+// four codes (a dword) as Kind, exactly
+template <typename Code, typename Kind> __device__ __forceinline__ void codes4(uint32_t c, uint32_t &lo, uint32_t &hi) {
+    if constexpr (std::is_same_v<Code, CodeE4M3> && std::is_same_v<Kind, __bf16>) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
+    } else if constexpr (std::is_same_v<Code, CodeE4M3>) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, true));
+    } else if constexpr (std::is_same_v<Kind, _Float16>) {
+        // 0x6400 + u is 1024 + u in f16, u = code + 128 < 256: exact, and so is the difference
+        const uint32_t u = c ^ 0x80808080u;
+        const f16x2_t off = {(_Float16)1152.f, (_Float16)1152.f};
+        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+    } else {
+        float x[4];
+        Code::decode(c, x);
+        lo = pack2<Kind>(x[0], x[1]);
+        hi = pack2<Kind>(x[2], x[3]);
+    }
+}
+template <typename Code, typename Kind> __device__ __forceinline__ u32x4 codes8(uint32_t a, uint32_t b) {
+    uint32_t w0, w1, w2, w3;
+    codes4<Code, Kind>(a, w0, w1);
+    codes4<Code, Kind>(b, w2, w3);
+    return u32x4{w0, w1, w2, w3};
+}
+// bytes of `w` that are an e4m3 NaN, as 0x80 in each
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// 16 codes without their NaNs; bit j of the result: code j was one
+__device__ __forceinline__ uint32_t drop_nans(u32x4 &v) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t b = nan_bytes(v[w]);
+        v[w] &= ~((b >> 7) * 0xffu);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= ((b >> (8 * e + 7)) & 1u) << (4 * w + e);
+    }
+    return found;
+}
+
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
+// A value scale: its logarithm, its reciprocal, and the factor of the probabilities that go with it: 1 but for zero, tiny and
+// negative scales.  One that is not finite counts as 1 here and makes the scores of its tokens NaN.
+struct ValueScale { float log, inv, factor; };
+__device__ __forceinline__ ValueScale value_scale(float vs) {
+    if (!finite(vs)) vs = 1.f;
+    const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
+    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f};
+}
+
+// ---- which tokens -------------------------------------------------------------------------------------------------------
+// The tokens [lo, hi) that row i of a sequence sees; nothing for a row that is none or has no place in the cache.
+struct Range { int lo, hi; };
+__device__ __forceinline__ Range row_range(const AttArgs &a, const KvSeq &s, int i) {
+    const int p = s.begin + i;
+    if (i >= s.n || p < 0) return {0, 0};
+    const int hi = a.causal && p + 1 < s.length ? p + 1 : s.length;
+    const int lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+    return {lo < hi ? lo : hi, hi};
+}
+// 64-token tiles that rows i0 .. i1 of a sequence see between them: [first, last)
+__device__ __forceinline__ void tile_range(const AttArgs &a, const KvSeq &s, int i0, int i1, int &first, int &last) {
+    if (i1 >= s.n) i1 = s.n - 1;
+    if (i0 + s.begin < 0) i0 = -s.begin;  // rows before token 0 see nothing
+    first = last = 0;
+    if (i0 > i1) return;
+    const Range x = row_range(a, s, i0), y = row_range(a, s, i1);  // both ends grow with the row
+    if (y.hi <= x.lo) return;
+    first = x.lo / 64;
+    last = (y.hi + 63) / 64;
+}
+// tiles in a slice when `tiles` of them are cut into at most `splits` slices: no fewer than kMinTiles
+constexpr int kMinTiles = 16;
+__device__ __forceinline__ int slice_tiles(int tiles, int splits) {
+    const int each = (tiles + splits - 1) / splits;
+    return each < kMinTiles ? kMinTiles : each;
+}
+// the part of [first, last) that slice `split` walks; false if there is none (slice 0 always has one, if empty)
+__device__ __forceinline__ bool slice_of(const AttArgs &a, int split, int &first, int &last) {
+    const int each = a.splits > 1 ? slice_tiles(last - first, a.splits) : last - first, b = first + split * each;
+    last = b + each < last ? b + each : last;
+    first = b;
+    return split == 0 || first < last;
+}
+// The table's entry for a token, read without a branch (past the last page: the last page's), and the page it stands for: -1 if
+// the token is not below the length or the entry is none.  Loads go to page 0 then, which exists (a sequence of a cache without
+// pages has length 0), and what they bring is masked.
+__device__ __forceinline__ int entry_at(const AttArgs &a, int seq, int token) {
+    const int slot = token >> a.kv.page_shift, at = slot < a.kv.pages_per_seq ? slot : a.kv.pages_per_seq - 1;
+    const int64_t k = (int64_t)seq * a.kv.pages_per_seq + at;
+    return a.kv.table ? a.kv.table[k] : (int)k;
+}
+__device__ __forceinline__ int page_of(const AttArgs &a, const KvSeq &s, int entry, int token) {
+    return token < s.length && (unsigned)entry < (unsigned)a.kv.num_pages ? entry : -1;
+}
+// eight values of a row as Kind parts; zeros past the end of the head
+template <typename T, int QP> __device__ __forceinline__ void load_query(const T *src, bool there, u32x4 (&q)[QP]) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    if (there) {
+        constexpr int V = kVecBytes / (int)sizeof(T);
+#pragma unroll
+        for (int p = 0; p < 8 / V; ++p) {
+            const vec_t<T, V> w = reinterpret_cast<const vec_t<T, V> *>(src)[p];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[p * V + e] = load_acc(w.v[e]);
+        }
+    }
+    split_parts<typename RowType<T>::Kind, QP>(x, q);
+}
+template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, float x1, float x2, float x3) {
+    const float y[4] = {x0, x1, x2, x3};
+    vec_t<T, 4> w;
+    store_acc_vec<T, 4>(w, y);
+    *reinterpret_cast<vec_t<T, 4> *>(dst) = w;
+}
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? kNone : kLn2 * (m - kLift + __builtin_amdgcn_logf(l)); }
+
+// ---- few rows -------------------------------------------------------------------------------------------------------------
+// One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile
+// and meet at the end.  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
+// loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes.
+template <typename T, typename Code, int SPANS, bool EXACT, bool ONE>
+static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
+    using Kind = typename RowType<T>::Kind;
+    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
+    __shared__ float meet_o[2][16][SPANS * 64 + 4];
+    __shared__ float meet_m[4][16], meet_l[4][16];
+    unsigned blk = blockIdx.x;
+    const int split = blk % (unsigned)a.splits; blk /= (unsigned)a.splits;
+    const int rt = blk % (unsigned)a.row_tiles; blk /= (unsigned)a.row_tiles;
+    const int head = blk % (unsigned)a.kv.heads, seq = blk / (unsigned)a.kv.heads;
+    const KvSeq s = kv_seq(a.kv, seq);
+    const int G = a.group, rows = s.n * G, r0 = rt * 16;
+    if (r0 >= rows) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int D = EXACT ? SPANS * 64 : a.kv.dim, P = a.kv.page_size;
+    int tile, tile_end;
+    tile_range(a, s, r0 / G, (r0 + 15) / G, tile, tile_end);
+    if (!slice_of(a, split, tile, tile_end)) return;  // the joining launch knows
+
+    // keys: row n of score tile t is token 16 (n / 4) + 4 t + n % 4; values and scales: tokens 16 g .. 16 g + 15
+    const int kofs = 16 * (n >> 2), gofs = 16 * g;
+    tile += wave;
+    u32x4 kc[4][SPANS], vc[DT];
+    int kentry = 0, gentry = 0, gp = -1;
+    float ks = 0.f, vs = 0.f;
+    // ONE: a tile lies in one page, whose number, address and scales are the same for all lanes and stay in scalar registers
+    auto entries = [&](int t) __attribute__((always_inline)) {
+        kentry = entry_at(a, seq, t * 64 + (ONE ? 0 : kofs));
+        gentry = ONE ? kentry : entry_at(a, seq, t * 64 + gofs);
+    };
+    const int64_t page_bytes = (int64_t)a.kv.heads * P * D;
+    const uint8_t *khead = a.kv.k + (int64_t)head * P * D, *vhead = a.kv.v + (int64_t)head * P * D;
+    const uint32_t kin = ((kofs & (P - 1)) + (n & 3)) * D, vin = gofs & (P - 1);
+    auto load_keys = [&](int t) __attribute__((always_inline)) {  // and the scales
+        const int half = (t * 64) & (P - 1) & 64;  // the second half of a page of 128
+        const int k = page_of(a, s, kentry, t * 64 + (ONE ? 0 : kofs));
+        gp = ONE ? k : page_of(a, s, gentry, t * 64 + gofs);
+        const uint8_t *src = khead + (k < 0 ? 0 : k) * page_bytes + half * D;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < SPANS; ++c) {
+                const int d = c * 64 + g * 16;  // past the end of the head the query is zero: any key of the row will do
+                kc[u][c] = *reinterpret_cast<const u32x4 *>(src + (kin + 4 * u * D + (EXACT || d < D ? d : 0)));
+            }
+        const int64_t at = (int64_t)(gp < 0 ? 0 : gp) * a.kv.heads + head;
+        ks = a.kv.k_scale[at];
+        vs = a.kv.v_scale[at];
+    };
+    auto load_values = [&](int t, int page) __attribute__((always_inline)) {
+        const uint8_t *src = vhead + (page < 0 ? 0 : page) * page_bytes + ((t * 64) & (P - 1) & 64);
+#pragma unroll
+        for (int u = 0; u < DT; ++u) {
+            const int d = u * 16 + n;  // dimensions past the end of the head are not stored
+            vc[u] = *reinterpret_cast<const u32x4 *>(src + (vin + (EXACT || d < D ? d : n) * P));
+        }
+    };
+    if (tile < tile_end) {
+        entries(tile);
+        load_keys(tile);
+        load_values(tile, gp);
+        entries(tile + 4);
+    }
+
+    // this lane's row
+    const int r = r0 + n, i = r / G, h = head * G + (r - i * G);
+    const bool real = r < rows;
+    Range vis = row_range(a, s, i);
+    if (!real) vis = {0, 0};
+    u32x4 q[SPANS * 2][QP];
+    {
+        const T *src = (const T *)a.q + (s.first + i) * a.q_row + h * a.q_head;
+#pragma unroll
+        for (int c = 0; c < SPANS * 2; ++c) {  // span c / 2, half c % 2
+            const int d = (c / 2) * 64 + g * 16 + (c % 2) * 8;
+            load_query<T, QP>(src + d, real && d < D, q[c]);
+        }
+    }
+    // a tile needs no masks when every real row sees all of it
+    const int last_row = (r0 + 15 < rows ? r0 + 15 : rows - 1) / G;
+    const int all_lo = row_range(a, s, last_row).lo, all_hi = row_range(a, s, r0 / G).hi;
+
+    float m = kNone, l = 0.f;
+    f32x4_t o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (; tile < tile_end; tile += 4) {
+        const int tok0 = tile * 64, gb = tok0 + gofs;
+        const ValueScale vsc = value_scale(vs);
+        const bool none = gp < 0, fine = finite(vs), more = tile + 4 < tile_end;
+        const float mul = ks * a.scale;
+        const bool odd = tok0 < all_lo || tok0 + 64 > all_hi || __any(none || !fine);
+        float sc[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < SPANS * 2; ++c) {
+                const u32x4 k = codes8<Code, Kind>(kc[t][c / 2][(c % 2) * 2], kc[t][c / 2][(c % 2) * 2 + 1]);
+#pragma unroll
+                for (int p = 0; p < QP; ++p) acc = mma16<Kind>(k, q[c][p], acc);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[4 * t + e] = __builtin_fmaf(acc[e], mul, vsc.log);
+        }
+        // the keys' registers are free: the next tile's keys come while this one's values are used
+        if (more) load_keys(tile + 4);
+        if (odd) {
+            uint32_t bad = fine ? 0u : 0xffffu;  // bit j: the score of token 16 g + j becomes NaN
+            if constexpr (std::is_same_v<Code, CodeE4M3>) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) any |= nan_bytes(vc[t][w]);
+                if (__any(any != 0)) {
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const uint32_t found = drop_nans(vc[t]);
+                        if (EXACT || t * 16 < D) bad |= found;
+                    }
+#pragma unroll
+                    for (int x = 1; x < 16; x <<= 1) bad |= __shfl_xor(bad, x, 16);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (bad >> e & 1u) sc[e] = __builtin_nanf("");
+                if (none || gb + e < vis.lo || gb + e >= vis.hi) sc[e] = kNone;
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, sc[e]);
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        float sum = 0.f;
+        u32x4 p[2][PP];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(sc[8 * u + e] - (base - kLift));
+                sum += x[e];
+                x[e] *= vsc.factor;
+            }
+            split_parts<_Float16, PP>(x, p[u]);
+        }
+        l = __builtin_fmaf(sum, vsc.inv, l * alpha);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            o[t] *= alpha;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const u32x4 v = codes8<Code, _Float16>(vc[t][2 * u], vc[t][2 * u + 1]);
+#pragma unroll
+                for (int k = 0; k < PP; ++k) o[t] = mma16<_Float16>(v, p[u][k], o[t]);
+            }
+        }
+        if (more) {
+            load_values(tile + 4, gp);
+            entries(tile + 8);
+        }
+    }
+
+    // the four waves meet: l over the lane groups, then everything relative to the common maximum, added in wave order
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) meet_m[wave][n] = m;
+    __syncthreads();
+    float top = meet_m[0][n];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, meet_m[w][n]);
+    const float base = top == kNone ? 0.f : top, mine = __builtin_amdgcn_exp2f(m - base);
+    l *= mine;
+    if (g == 0) meet_l[wave][n] = l;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] *= mine;
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {  // waves 2, 3 give to 0, 1; then 1 to 0
+        if (wave >= half && wave < 2 * half)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t *>(&meet_o[wave - half][n][t * 16 + g * 4]) = o[t];
+        __syncthreads();
+        if (wave < half)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] += *reinterpret_cast<const f32x4_t *>(&meet_o[wave][n][t * 16 + g * 4]);
+        __syncthreads();
+    }
+    if (wave != 0 || !real) return;
+    l = (meet_l[0][n] + meet_l[1][n]) + (meet_l[2][n] + meet_l[3][n]);
+    const int64_t at = (s.first + i) * a.q_heads + h;
+    if (a.splits > 1) {
+        const int64_t slot = (int64_t)split * a.kv.rows * a.q_heads + at;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            if (t * 16 < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + t * 16 + g * 4) = o[t];
+        if (g == 0) { a.part_ml[2 * slot] = top; a.part_ml[2 * slot + 1] = l; }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+        if (t * 16 < D) store4<T>(dst + t * 16 + g * 4, o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv);
+    if (g == 0 && a.lse) a.lse[at] = lse_of(top, l);
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------------------------
+// One workgroup: 32 rows a wave of one (sequence, key head); the waves share every 64-token tile, whose codes are turned into
+// 16-bit operands once, on their way from registers (loaded a tile ahead) into LDS.  Scores: two 32-token products of
+// 32x32x16; row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
+// their probabilities to the second product as they are.  Rows of LDS are padded by 16 bytes: 16 lanes that read 16 bytes at
+// one column of 16 rows meet 16 different bank groups.  Bound by the matrix pipe and the vector pipe's 2^x.
+template <typename T, typename Code, int DP, bool EXACT, bool ONE, int WAVES>
+static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>::QP == 1) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
+    using Kind = typename RowType<T>::Kind;
+    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = DP / 32, THREADS = WAVES * kWave;
+    constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, PIECES = (DP * 4 + THREADS - 1) / THREADS;
+    __shared__ __attribute__((aligned(16))) unsigned char kl[64 * KPITCH], vl[DP * VPITCH];
+    __shared__ uint32_t bad_tokens[2][2];
+    // longest tiles of rows first; the tiles of one (sequence, head) stay on one XCD when there are a multiple of 8 pairs
+    const unsigned pairs = (unsigned)a.kv.batch * a.kv.heads;
+    unsigned blk = blockIdx.x;
+    const int pair = blk % pairs; blk /= pairs;
+    const int split = blk % (unsigned)a.splits, rt = a.row_tiles - 1 - (int)(blk / (unsigned)a.splits);
+    const int head = pair % a.kv.heads, seq = pair / a.kv.heads;
+    const KvSeq s = kv_seq(a.kv, seq);
+    const int G = a.group, rows = s.n * G, r0 = rt * (WAVES * 32);
+    if (r0 >= rows) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h2 = lane >> 5;
+    const int D = EXACT ? DP : a.kv.dim, P = a.kv.page_size;
+    int tile, tile_end;
+    tile_range(a, s, r0 / G, (r0 + WAVES * 32 - 1) / G, tile, tile_end);
+    if (!slice_of(a, split, tile, tile_end)) return;
+
+    // pieces of 16 codes that this thread brings: of the keys token kt, dimensions kd ..; of the values dimension vd, tokens vt ..
+    int kt[PIECES], kd[PIECES], vd[PIECES], vt[PIECES];
+    uint32_t kofs[PIECES], vofs[PIECES];  // where the pieces lie in a page of this head, for tiles that begin in a page's first 64 tokens
+    bool there[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const int id = threadIdx.x + j * THREADS, per = D / 16;
+        there[j] = EXACT || id < 4 * D;  // others load piece 0 and drop it
+        const int x = there[j] ? id : 0;
+        kt[j] = x / per;
+        kd[j] = (x - kt[j] * per) * 16;
+        // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
+        vd[j] = P == 16 ? x % D : x >> 2;
+        vt[j] = (P == 16 ? x / D : x & 3) * 16;
+        kofs[j] = (kt[j] & (P - 1)) * D + kd[j];
+        vofs[j] = vd[j] * P + (vt[j] & (P - 1));
+    }
+    if (threadIdx.x < 4) bad_tokens[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    if (D < DP) {  // what pads the head stays zero
+        for (int id = threadIdx.x; id < 64 * (DP - D) / 8; id += THREADS)
+            *reinterpret_cast<u32x4 *>(kl + (id / ((DP - D) / 8)) * KPITCH + D * 2 + (id % ((DP - D) / 8)) * 16) = u32x4{0u, 0u, 0u, 0u};
+        for (int id = threadIdx.x; id < (DP - D) * 8; id += THREADS) *reinterpret_cast<u32x4 *>(vl + (D + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
+
+    // this lane's row
+    const int w0 = r0 + wave * 32, r = w0 + n, i = r / G, h = head * G + (r - i * G);
+    const bool real = r < rows;
+    Range vis = row_range(a, s, i);
+    if (!real) vis = {0, 0};
+    u32x4 q[DP / 16][QP];
+    {
+        const T *src = (const T *)a.q + (s.first + i) * a.q_row + h * a.q_head;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) load_query<T, QP>(src + c * 16 + h2 * 8, real && c * 16 < D, q[c]);
+    }
+    // tokens that any row of the wave sees, that all of them see; that all rows of the workgroup see
+    Range any = {0, 0}, all = {0, 0}, group_all;
+    {
+        const int last = (r0 + WAVES * 32 < rows ? r0 + WAVES * 32 : rows) - 1, wlast = w0 + 31 < rows ? w0 + 31 : rows - 1;
+        group_all = {row_range(a, s, last / G).lo, row_range(a, s, r0 / G).hi};
+        if (w0 < rows) {
+            const Range x = row_range(a, s, w0 / G), y = row_range(a, s, wlast / G);
+            any = {x.lo, y.hi};
+            all = {y.lo, x.hi};
+        }
+    }
+
+    float m = kNone, l = 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+
+    // table entries two tiles ahead, codes and scales one.  ONE: a tile lies in one page, whose number, address and scales are the
+    // same for all lanes and stay in scalar registers.
+    constexpr int E = ONE ? 1 : PIECES, S = ONE ? 1 : 2;
+    int kentry[E], ventry[E], sentry[S], sp[S];
+    bool vnone[E];
+    u32x4 kc[PIECES], vc[PIECES];
+    float ks_next[S], vs_next[S];
+    auto entries = [&](int t) __attribute__((always_inline)) {
+        if constexpr (ONE) {
+            kentry[0] = entry_at(a, seq, t * 64);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                kentry[j] = entry_at(a, seq, t * 64 + kt[j]);
+                ventry[j] = entry_at(a, seq, t * 64 + vt[j]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sentry[u] = entry_at(a, seq, t * 64 + u * 32 + h2 * 16);
+        }
+    };
+    const int64_t page_bytes = (int64_t)a.kv.heads * P * D;
+    const uint8_t *khead = a.kv.k + (int64_t)head * P * D, *vhead = a.kv.v + (int64_t)head * P * D;
+    auto fetch = [&](int t) __attribute__((always_inline)) {
+        const int half = (t * 64) & (P - 1) & 64;  // the second half of a page of 128
+        if constexpr (ONE) {
+            sp[0] = page_of(a, s, kentry[0], t * 64);
+            vnone[0] = sp[0] < 0;
+            const int page = sp[0] < 0 ? 0 : sp[0];
+            const uint8_t *ksrc = khead + page * page_bytes + half * D, *vsrc = vhead + page * page_bytes + half;
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                kc[j] = *reinterpret_cast<const u32x4 *>(ksrc + kofs[j]);
+                vc[j] = *reinterpret_cast<const u32x4 *>(vsrc + vofs[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                const int kp = page_of(a, s, kentry[j], t * 64 + kt[j]), vp = page_of(a, s, ventry[j], t * 64 + vt[j]);
+                vnone[j] = vp < 0;
+                kc[j] = *reinterpret_cast<const u32x4 *>(khead + (kp < 0 ? 0 : kp) * page_bytes + (kofs[j] + half * D));
+                vc[j] = *reinterpret_cast<const u32x4 *>(vhead + (vp < 0 ? 0 : vp) * page_bytes + (vofs[j] + half));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sp[u] = page_of(a, s, sentry[u], t * 64 + u * 32 + h2 * 16);
+        }
+#pragma unroll
+        for (int u = 0; u < S; ++u) {
+            const int64_t at = (int64_t)(sp[u] < 0 ? 0 : sp[u]) * a.kv.heads + head;
+            ks_next[u] = a.kv.k_scale[at];
+            vs_next[u] = a.kv.v_scale[at];
+        }
+    };
+    if (tile < tile_end) {
+        entries(tile);
+        fetch(tile);
+        entries(tile + 1);
+    }
+    const int krow = (16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3)) * KPITCH + h2 * 16, vrow = n * VPITCH + h2 * 32;
+    __syncthreads();
+    for (; tile < tile_end; ++tile) {
+        const int tok0 = tile * 64, slot = tile & 1;
+        const bool group_masked = tok0 < group_all.lo || tok0 + 64 > group_all.hi;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            if (!there[j]) continue;
+            u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
+            dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
+            dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
+            if constexpr (std::is_same_v<Code, CodeE4M3>) {
+                if (vnone[ONE ? 0 : j]) vc[j] = u32x4{0u, 0u, 0u, 0u};
+                if (group_masked) {
+                    const uint32_t found = drop_nans(vc[j]);
+                    if (found) atomicOr(&bad_tokens[slot][vt[j] >> 5], found << (vt[j] & 16));
+                }
+            }
+            dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
+            dst[0] = codes8<Code, _Float16>(vc[j][0], vc[j][1]);
+            dst[1] = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
+        }
+        float ks[2], vs[2];
+        int page[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) { ks[u] = ks_next[ONE ? 0 : u] * a.scale; vs[u] = vs_next[ONE ? 0 : u]; page[u] = sp[ONE ? 0 : u]; }
+        if (tile + 1 < tile_end) {
+            fetch(tile + 1);
+            entries(tile + 2);
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) bad_tokens[slot ^ 1][threadIdx.x] = 0;
+        if (tok0 < any.hi && tok0 + 64 > any.lo) {
+            f32x16 sc[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    const u32x4 k = *reinterpret_cast<const u32x4 *>(kl + krow + u * 32 * KPITCH + c * 32);
+#pragma unroll
+                    for (int p = 0; p < QP; ++p) sc[u] = mma32<Kind>(k, q[c][p], sc[u]);
+                }
+            }
+            const ValueScale vsc[2] = {value_scale(vs[0]), value_scale(vs[1])};
+            const uint32_t bad0 = bad_tokens[slot][0], bad1 = bad_tokens[slot][1];
+            const bool odd = tok0 < all.lo || tok0 + 64 > all.hi || (bad0 | bad1) ||
+                             __any(page[0] < 0 || page[1] < 0 || !(ks[0] >= 0.f) || !(ks[1] >= 0.f) || !finite(vs[0]) || !finite(vs[1]) || vsc[0].factor != 1.f || vsc[1].factor != 1.f);
+            float top = m;
+            if (odd) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t bad = finite(vs[u]) ? (u ? bad1 : bad0) >> (16 * h2) : 0xffffu;
+                    const int t0 = tok0 + u * 32 + h2 * 16;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float x = __builtin_fmaf(sc[u][e], ks[u], vsc[u].log);
+                        if (bad >> e & 1u) x = __builtin_nanf("");
+                        if (page[u] < 0 || t0 + e < vis.lo || t0 + e >= vis.hi) x = kNone;
+                        sc[u][e] = x;
+                        top = __builtin_fmaxf(top, x);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x = sc[u][0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[u][e]);
+                    top = __builtin_fmaxf(top, __builtin_fmaf(x, ks[u], vsc[u].log));  // ks >= 0: the largest product is the largest score
+                }
+            }
+            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+            const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l *= alpha;
+            u32x4 p[2][2][PP];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // the scores are there already (mul 1, add 0) or still to be made from the products
+                const float mul = odd ? 1.f : ks[u], add = (odd ? 0.f : vsc[u].log) - (base - kLift);
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * v + e], mul, add));
+                        sum += x[e];
+                    }
+                    if (odd)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] *= vsc[u].factor;
+                    split_parts<_Float16, PP>(x, p[u][v]);
+                }
+                l = __builtin_fmaf(sum, vsc[u].inv, l);
+            }
+            if (__any(alpha != 1.f)) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[t] *= alpha;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + vrow + t * 32 * VPITCH + u * 64 + v * 16);
+#pragma unroll
+                        for (int k = 0; k < PP; ++k) o[t] = mma32<_Float16>(x, p[u][v][k], o[t]);
+                    }
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    if (!real) return;
+    const int64_t at = (s.first + i) * a.q_heads + h;
+    if (a.splits > 1) {
+        const int64_t slot = (int64_t)split * a.kv.rows * a.q_heads + at;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int d = t * 32 + b * 8 + h2 * 4;
+                if (d < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + d) = f32x4_t{o[t][4 * b], o[t][4 * b + 1], o[t][4 * b + 2], o[t][4 * b + 3]};
+            }
+        if (h2 == 0) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = t * 32 + b * 8 + h2 * 4;
+            if (d < D) store4<T>(dst + d, o[t][4 * b] * inv, o[t][4 * b + 1] * inv, o[t][4 * b + 2] * inv, o[t][4 * b + 3] * inv);
+        }
+    if (h2 == 0 && a.lse) a.lse[at] = lse_of(m, l);
+}
+
+// ---- the slices of a row ------------------------------------------------------------------------------------------------
+// One workgroup for a packed row and query head.  Groups of dim / 4 lanes (rounded up to a power of two) take every so many-th
+// slice, each in one pass with a running maximum, and meet in LDS; the group's sums are added in group order.
+template <typename T>
+static __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs a) {
+    __shared__ f32x4_t meet_o[kBlock];
+    __shared__ float meet_m[16], meet_l[16];
+    unsigned blk = blockIdx.x;
+    const int h = blk % (unsigned)a.q_heads; blk /= (unsigned)a.q_heads;
+    const int i = blk % (unsigned)a.kv.max_rows, seq = blk / (unsigned)a.kv.max_rows;
+    const KvSeq s = kv_seq(a.kv, seq);
+    if (i >= s.n) return;
+    const int r0 = (i * a.group + h % a.group) / a.tile_rows * a.tile_rows;
+    int first, last;
+    tile_range(a, s, r0 / a.group, (r0 + a.tile_rows - 1) / a.group, first, last);
+    const int each = slice_tiles(last - first, a.splits), used = last > first ? (last - first + each - 1) / each : 1;
+    const int64_t at = (s.first + i) * a.q_heads + h, pitch = a.kv.rows * a.q_heads;
+    const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64, groups = kBlock / lanes, group = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
+    const bool live = d < a.kv.dim;
+    const float *po = a.part_o + at * a.kv.dim + (live ? d : 0), *pm = a.part_ml + 2 * at;
+    float m = kNone, l = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = group; k < used; k += groups) {
+        const f32x4_t x = *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim);
+        const float mk = pm[2 * k * pitch], lk = pm[2 * k * pitch + 1];
+        const float top = __builtin_fmaxf(m, mk), base = top == kNone ? 0.f : top;
+        const float wa = __builtin_amdgcn_exp2f(m - base), wb = __builtin_amdgcn_exp2f(mk - base);
+        o = o * wa + x * wb;
+        l = __builtin_fmaf(l, wa, lk * wb);
+        m = top;
+    }
+    meet_o[threadIdx.x] = o;
+    if (threadIdx.x % lanes == 0) { meet_m[group] = m; meet_l[group] = l; }
+    __syncthreads();
+    if (group > 0) return;
+    float top = m;
+    for (int k = 1; k < groups; ++k) top = __builtin_fmaxf(top, meet_m[k]);
+    const float base = top == kNone ? 0.f : top;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+    for (int k = 0; k < groups; ++k) {
+        const float w = __builtin_amdgcn_exp2f(meet_m[k] - base);
+        o += meet_o[k * lanes + threadIdx.x] * w;
+        l = __builtin_fmaf(meet_l[k], w, l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (threadIdx.x == 0 && a.lse) a.lse[at] = lse_of(top, l);
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+constexpr int kWaves = 4, kTileRows = kWaves * 32;
+template <typename T, typename Code, int SPANS, bool EXACT, bool ONE> void launch_one(const AttArgs &a, hipStream_t st) {
+    const unsigned blocks = (unsigned)((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits);
+    if (a.tile_rows == 16) kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE><<<blocks, kBlock, 0, st>>>(a);
+    else kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+}
+// head sizes that fill their registers need no bounds in the loops, pages of at least 64 tokens no page number a lane
+template <typename T, typename Code, int SPANS> void launch_dim(const AttArgs &a, hipStream_t st) {
+    if (a.kv.dim != SPANS * 64) launch_one<T, Code, SPANS, false, false>(a, st);
+    else if (a.kv.page_size < 64) launch_one<T, Code, SPANS, true, false>(a, st);
+    else launch_one<T, Code, SPANS, true, true>(a, st);
+}
+template <typename T, typename Code> int kvattention_launch(const AttArgs &a, hipStream_t st) {
+    if (a.kv.dim <= 64) launch_dim<T, Code, 1>(a, st);
+    else if (a.kv.dim <= 128) launch_dim<T, Code, 2>(a, st);
+    else launch_dim<T, Code, 4>(a, st);
+    const int rc = launch_status();
+    if (rc != DXH_OK || a.splits == 1) return rc;
+    kvattention_join_kernel<T><<<(unsigned)((int64_t)a.kv.batch * a.kv.max_rows * a.q_heads), kBlock, 0, st>>>(a);
+    return launch_status();
+}
+
+// one source file a row type: they compile side by side
+int kvattention_f32(const AttArgs &a, bool i8, hipStream_t st);
+int kvattention_f16(const AttArgs &a, bool i8, hipStream_t st);
+int kvattention_bf16(const AttArgs &a, bool i8, hipStream_t st);
+
+}  // namespace dxh

@@ -37,7 +37,7 @@ __device__ __forceinline__ bool tile_of_block(const RowsArgs &a, int &which, int
 }
 
 template <typename VT> __device__ __forceinline__ void store_row(VT *p, const VT &v, int nt) {
-    if (nt) st_mode<1>(p, v); else *p = v;
+    if (nt) st_mode<3>(p, v); else *p = v;
 }
 
 template <int THREADS> __device__ __forceinline__ uint32_t block_max(uint32_t v) {

@@ -74,6 +74,9 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     a.scale = scale * kLog2e;
     a.causal = causal;
     a.window = window > INT32_MAX ? 0 : (int)window;
+    // A cache of twice the last-level cache is not in it from step to step: 1.2 GB of codes 227 us plain, 216 with nt loads (268 MB: 57
+    // and 62).  Several tiles of rows read the codes more than once.
+    a.nt = a.tile_rows == 16 && a.row_tiles == 1 && (int64_t)2 * a.kv.num_pages * a.kv.heads * a.kv.page_size * a.kv.dim > ((int64_t)512 << 20);
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + (size_t)a.splits * a.kv.rows * q_heads * a.kv.dim;
     hipStream_t st = as_stream(stream);

@@ -34,11 +34,16 @@ struct AttArgs {
     float *lse, *part_o, *part_ml;  // partials: [slice][packed row][q head][dim] and [slice][packed row][q head][2]
     float scale;                    // scale * log2(e)
     int q_heads, group, causal, window, splits, row_tiles, tile_rows;
+    int nt;  // few rows and pages of at least 64 tokens: the codes are read past the last-level cache
 };
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 constexpr float kNone = -__builtin_inff();
 constexpr float kLift = 15.f;        // probabilities are held 2^15 times as large: at most 2^15 in f16, whose largest number is 65504
+// With 128-row tiles and one-part probabilities the reference of a row follows its maximum only when that has grown by more than
+// kSlack (in powers of two): the output is then rescaled in few tiles, and a probability, held 2^(15 - kSlack) times as large, is
+// still at most 2^15.
+constexpr float kSlack = 8.f;
 constexpr float kTinyScale = 0x1p-100f;  // value scales below it are multiplied into the codes: 1 / scale stays finite
 
 // ---- products ---------------------------------------------------------------------------------------------------------
@@ -121,6 +126,11 @@ __device__ __forceinline__ uint32_t drop_nans(u32x4 &v) {
     return found;
 }
 
+// the larger of a lane's value and that of lane ^ 32
+__device__ __forceinline__ float other_half_max(float x) {
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(float_to_bits(x), float_to_bits(x), false, false));
+    return __builtin_fmaxf(bits_to_float(r[0]), bits_to_float(r[1]));
+}
 __device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
 // A value scale: its logarithm, its reciprocal, and the factor of the probabilities that go with it: 1 but for zero, tiny and
 // negative scales.  One that is not finite counts as 1 here and makes the scores of its tokens NaN.
@@ -129,6 +139,17 @@ __device__ __forceinline__ ValueScale value_scale(float vs) {
     if (!finite(vs)) vs = 1.f;
     const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
     return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f};
+}
+// Where a scale is so much smaller than the largest so far that 2^(t - m) could be 0 while the token's share of l is not (a page of
+// zeros beside one of huge values), the exponent keeps within kReach of that largest one's and the rest of the scale becomes a
+// factor.  What it is a factor of is then below 2^-85 of the largest values.
+constexpr float kReach = 85.f;
+__device__ __forceinline__ bool out_of_reach(const ValueScale &v, float largest) { return v.log < largest - kReach; }
+__device__ __forceinline__ void reach(ValueScale &v, float largest) {
+    if (!out_of_reach(v, largest)) return;
+    v.factor *= __builtin_amdgcn_exp2f(v.log - (largest - kReach));
+    v.inv = __builtin_amdgcn_exp2f(kReach - largest);
+    v.log = largest - kReach;
 }
 
 // ---- which tokens -------------------------------------------------------------------------------------------------------
@@ -198,13 +219,14 @@ template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, f
     store_acc_vec<T, 4>(w, y);
     *reinterpret_cast<vec_t<T, 4> *>(dst) = w;
 }
-__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? kNone : kLn2 * (m - kLift + __builtin_amdgcn_logf(l)); }
+// `ref`: the power of two that l (and the output) are counted in
+__device__ __forceinline__ float lse_of(float ref, float l) { return l == 0.f ? kNone : kLn2 * (ref + __builtin_amdgcn_logf(l)); }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
 // One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile
 // and meet at the end.  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
 // loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes.
-template <typename T, typename Code, int SPANS, bool EXACT, bool ONE>
+template <typename T, typename Code, int SPANS, bool EXACT, bool ONE, bool NT>
 static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
@@ -247,7 +269,8 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
 #pragma unroll
             for (int c = 0; c < SPANS; ++c) {
                 const int d = c * 64 + g * 16;  // past the end of the head the query is zero: any key of the row will do
-                kc[u][c] = *reinterpret_cast<const u32x4 *>(src + (kin + 4 * u * D + (EXACT || d < D ? d : 0)));
+                const u32x4 *p = reinterpret_cast<const u32x4 *>(src + (kin + 4 * u * D + (EXACT || d < D ? d : 0)));
+                kc[u][c] = ld_sel<NT>(p);
             }
         const int64_t at = (int64_t)(gp < 0 ? 0 : gp) * a.kv.heads + head;
         ks = a.kv.k_scale[at];
@@ -258,7 +281,8 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
 #pragma unroll
         for (int u = 0; u < DT; ++u) {
             const int d = u * 16 + n;  // dimensions past the end of the head are not stored
-            vc[u] = *reinterpret_cast<const u32x4 *>(src + (vin + (EXACT || d < D ? d : n) * P));
+            const u32x4 *p = reinterpret_cast<const u32x4 *>(src + (vin + (EXACT || d < D ? d : n) * P));
+            vc[u] = ld_sel<NT>(p);
         }
     };
     if (tile < tile_end) {
@@ -286,14 +310,23 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
     const int last_row = (r0 + 15 < rows ? r0 + 15 : rows - 1) / G;
     const int all_lo = row_range(a, s, last_row).lo, all_hi = row_range(a, s, r0 / G).hi;
 
-    float m = kNone, l = 0.f;
+    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale
     f32x4_t o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     for (; tile < tile_end; tile += 4) {
         const int tok0 = tile * 64, gb = tok0 + gofs;
-        const ValueScale vsc = value_scale(vs);
+        ValueScale vsc = value_scale(vs);
+        {
+            float x = gp < 0 ? kNone : vsc.log;
+            if constexpr (!ONE) {
+                x = __builtin_fmaxf(x, __shfl_xor(x, 16));
+                x = __builtin_fmaxf(x, __shfl_xor(x, 32));
+            }
+            largest = __builtin_fmaxf(largest, x);
+            reach(vsc, largest);
+        }
         const bool none = gp < 0, fine = finite(vs), more = tile + 4 < tile_end;
         const float mul = ks * a.scale;
         const bool odd = tok0 < all_lo || tok0 + 64 > all_hi || __any(none || !fine);
@@ -405,7 +438,7 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             if (t * 16 < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + t * 16 + g * 4) = o[t];
-        if (g == 0) { a.part_ml[2 * slot] = top; a.part_ml[2 * slot + 1] = l; }
+        if (g == 0) { a.part_ml[2 * slot] = top - kLift; a.part_ml[2 * slot + 1] = l; }
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -413,20 +446,25 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
 #pragma unroll
     for (int t = 0; t < DT; ++t)
         if (t * 16 < D) store4<T>(dst + t * 16 + g * 4, o[t][0] * inv, o[t][1] * inv, o[t][2] * inv, o[t][3] * inv);
-    if (g == 0 && a.lse) a.lse[at] = lse_of(top, l);
+    if (g == 0 && a.lse) a.lse[at] = lse_of(top - kLift, l);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------
 // One workgroup: 32 rows a wave of one (sequence, key head); the waves share every 64-token tile, whose codes are turned into
-// 16-bit operands once, on their way from registers (loaded a tile ahead) into LDS.  Scores: two 32-token products of
-// 32x32x16; row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
+// 16-bit operands once, on their way from registers (loaded a tile ahead) into LDS.  Scores: two 32-token products of 32x32x16;
+// row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
 // their probabilities to the second product as they are.  Rows of LDS are padded by 16 bytes: 16 lanes that read 16 bytes at
-// one column of 16 rows meet 16 different bank groups.  Bound by the matrix pipe and the vector pipe's 2^x.
+// one column of 16 rows meet 16 different bank groups.
+// Bound by the vector pipe and what it cannot hide: causal prompts of 4 x 3.3k-4.1k tokens, 32 / 8 heads of 128, 640 us (760
+// TFLOP/s), matrix pipe busy 31 %, vector pipe 45 % (2^x a third of that), waves waiting 34 %.  Eight waves a workgroup, two
+// buffers with one barrier a tile, an enforced alternation of matrix and vector instructions, and raised wave priority under
+// the products were measured at 682, 672, 669 and 674 us.
 template <typename T, typename Code, int DP, bool EXACT, bool ONE, int WAVES>
 static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>::QP == 1) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = DP / 32, THREADS = WAVES * kWave;
     constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, PIECES = (DP * 4 + THREADS - 1) / THREADS;
+    constexpr float slack = PP == 1 ? kSlack : 0.f, lift = kLift - slack;
     __shared__ __attribute__((aligned(16))) unsigned char kl[64 * KPITCH], vl[DP * VPITCH];
     __shared__ uint32_t bad_tokens[2][2];
     // longest tiles of rows first; the tiles of one (sequence, head) stay on one XCD when there are a multiple of 8 pairs
@@ -465,7 +503,8 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
     if (D < DP) {  // what pads the head stays zero
         for (int id = threadIdx.x; id < 64 * (DP - D) / 8; id += THREADS)
             *reinterpret_cast<u32x4 *>(kl + (id / ((DP - D) / 8)) * KPITCH + D * 2 + (id % ((DP - D) / 8)) * 16) = u32x4{0u, 0u, 0u, 0u};
-        for (int id = threadIdx.x; id < (DP - D) * 8; id += THREADS) *reinterpret_cast<u32x4 *>(vl + (D + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
+        for (int id = threadIdx.x; id < (DP - D) * 8; id += THREADS)
+            *reinterpret_cast<u32x4 *>(vl + (D + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
     }
 
     // this lane's row
@@ -491,7 +530,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
         }
     }
 
-    float m = kNone, l = 0.f;
+    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale
     f32x16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -502,7 +541,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
     // same for all lanes and stay in scalar registers.
     constexpr int E = ONE ? 1 : PIECES, S = ONE ? 1 : 2;
     int kentry[E], ventry[E], sentry[S], sp[S];
-    bool vnone[E];
+    bool vnone[E];  // values: the page is none
     u32x4 kc[PIECES], vc[PIECES];
     float ks_next[S], vs_next[S];
     auto entries = [&](int t) __attribute__((always_inline)) {
@@ -550,125 +589,169 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
             vs_next[u] = a.kv.v_scale[at];
         }
     };
-    if (tile < tile_end) {
-        entries(tile);
-        fetch(tile);
-        entries(tile + 1);
-    }
     const int krow = (16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3)) * KPITCH + h2 * 16, vrow = n * VPITCH + h2 * 32;
-    __syncthreads();
-    for (; tile < tile_end; ++tile) {
-        const int tok0 = tile * 64, slot = tile & 1;
-        const bool group_masked = tok0 < group_all.lo || tok0 + 64 > group_all.hi;
+    auto clean = [&](int t) __attribute__((always_inline)) {  // e4m3: values without NaNs where a mask or a missing page could meet them
+        if constexpr (std::is_same_v<Code, CodeE4M3>) {
+            bool gone = false;
+#pragma unroll
+            for (int j = 0; j < E; ++j) gone = gone || vnone[j];
+            const bool cut = t * 64 < group_all.lo || t * 64 + 64 > group_all.hi;
+            if (cut || __any(gone)) {
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) {
+                    if (!there[j]) continue;
+                    if (vnone[ONE ? 0 : j]) vc[j] = u32x4{0u, 0u, 0u, 0u};
+                    const uint32_t found = cut ? drop_nans(vc[j]) : 0u;
+                    if (found) atomicOr(&bad_tokens[t & 1][vt[j] >> 5], found << (vt[j] & 16));
+                }
+            }
+        }
+    };
+    // the codes in the registers as operands into LDS
+    auto stage = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             if (!there[j]) continue;
             u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
             dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
             dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
-            if constexpr (std::is_same_v<Code, CodeE4M3>) {
-                if (vnone[ONE ? 0 : j]) vc[j] = u32x4{0u, 0u, 0u, 0u};
-                if (group_masked) {
-                    const uint32_t found = drop_nans(vc[j]);
-                    if (found) atomicOr(&bad_tokens[slot][vt[j] >> 5], found << (vt[j] & 16));
-                }
-            }
             dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
             dst[0] = codes8<Code, _Float16>(vc[j][0], vc[j][1]);
             dst[1] = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
         }
-        float ks[2], vs[2];
-        int page[2];
+    };
+    __syncthreads();  // the zeroed flags and pads
+    if (tile < tile_end) {
+        entries(tile);
+        fetch(tile);
+        entries(tile + 1);
+    }
+    for (; tile < tile_end; ++tile) {
+        const int tok0 = tile * 64, slot = tile & 1;
+        const unsigned char *kb = kl + krow, *vb = vl + vrow;
+        clean(tile);
+        stage();
+        float ks[S], vs[S];
+        int page[S];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) { ks[u] = ks_next[ONE ? 0 : u] * a.scale; vs[u] = vs_next[ONE ? 0 : u]; page[u] = sp[ONE ? 0 : u]; }
+        for (int u = 0; u < S; ++u) { ks[u] = ks_next[u] * a.scale; vs[u] = vs_next[u]; page[u] = sp[u]; }
         if (tile + 1 < tile_end) {
             fetch(tile + 1);
             entries(tile + 2);
         }
-        __syncthreads();
+        __syncthreads();  // this tile is in LDS
         if (threadIdx.x < 2) bad_tokens[slot ^ 1][threadIdx.x] = 0;
-        if (tok0 < any.hi && tok0 + 64 > any.lo) {
-            f32x16 sc[2];
+        const bool cut = tok0 < group_all.lo || tok0 + 64 > group_all.hi;
+        ValueScale vsc[S];
+        bool plain = !cut;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < S; ++u) vsc[u] = value_scale(vs[u]);
+        {
+            float x = page[0] < 0 ? kNone : vsc[0].log;
+            if constexpr (!ONE) x = other_half_max(__builtin_fmaxf(x, page[S - 1] < 0 ? kNone : vsc[S - 1].log));
+            largest = __builtin_fmaxf(largest, x);
+        }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+        for (int u = 0; u < S; ++u) {
+            plain = plain && !__any(page[u] < 0 || !(ks[u] >= 0.f) || !finite(vs[u]) || vsc[u].factor != 1.f || out_of_reach(vsc[u], largest));
+        }
+        f32x16 sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+        auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c) {
-                    const u32x4 k = *reinterpret_cast<const u32x4 *>(kl + krow + u * 32 * KPITCH + c * 32);
+                    const u32x4 k = *reinterpret_cast<const u32x4 *>(kb + u * 32 * KPITCH + c * 32);
 #pragma unroll
                     for (int p = 0; p < QP; ++p) sc[u] = mma32<Kind>(k, q[c][p], sc[u]);
                 }
+        };
+        u32x4 p[2][2][PP];
+        auto powers = [&](int u, float mul, float add, float factor) __attribute__((always_inline)) {
+            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * v + e], mul, add));
+                    sum += x[e];
+                    x[e] *= factor;
+                }
+                split_parts<_Float16, PP>(x, p[u][v]);
             }
-            const ValueScale vsc[2] = {value_scale(vs[0]), value_scale(vs[1])};
-            const uint32_t bad0 = bad_tokens[slot][0], bad1 = bad_tokens[slot][1];
-            const bool odd = tok0 < all.lo || tok0 + 64 > all.hi || (bad0 | bad1) ||
-                             __any(page[0] < 0 || page[1] < 0 || !(ks[0] >= 0.f) || !(ks[1] >= 0.f) || !finite(vs[0]) || !finite(vs[1]) || vsc[0].factor != 1.f || vsc[1].factor != 1.f);
-            float top = m;
-            if (odd) {
+            l = __builtin_fmaf(sum, vsc[ONE ? 0 : u].inv, l);
+        };
+        auto outputs = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(vb + t * 32 * VPITCH + u * 64 + v * 16);
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) o[t] = mma32<_Float16>(x, p[u][v][k], o[t]);
+                }
+        };
+        auto follow = [&](float top) __attribute__((always_inline)) {  // the row's reference after scores of at most `top`
+            top = __builtin_fmaxf(m, top);
+            const bool move = top > m + slack;
+            if (__any(move)) {
+                const float to = move ? top : m, alpha = __builtin_amdgcn_exp2f(m - (to == kNone ? 0.f : to));
+                m = to;
+                l *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[t] *= alpha;
+            }
+        };
+        if (plain) {
+            scores();
+            float top = kNone;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x = sc[u][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[u][e]);
+                top = __builtin_fmaxf(top, __builtin_fmaf(x, ks[ONE ? 0 : u], vsc[ONE ? 0 : u].log));  // ks >= 0: the largest product is the largest score
+            }
+            follow(other_half_max(top));
+            powers(0, ks[0], vsc[0].log - (m - lift), 1.f);
+            outputs(0);
+            powers(1, ks[S - 1], vsc[S - 1].log - (m - lift), 1.f);
+            outputs(1);
+        } else {
+            if (tok0 < any.hi && tok0 + 64 > any.lo) {
+#pragma unroll
+                for (int u = 0; u < S; ++u) reach(vsc[u], largest);
+                scores();
+                const uint32_t bads[2] = {bad_tokens[slot][0], bad_tokens[slot][1]};
+                float top = kNone;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const uint32_t bad = finite(vs[u]) ? (u ? bad1 : bad0) >> (16 * h2) : 0xffffu;
+                    const int su = ONE ? 0 : u;
+                    const uint32_t bad = finite(vs[su]) ? bads[u] >> (16 * h2) : 0xffffu;
                     const int t0 = tok0 + u * 32 + h2 * 16;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float x = __builtin_fmaf(sc[u][e], ks[u], vsc[u].log);
+                        float x = __builtin_fmaf(sc[u][e], ks[su], vsc[su].log);
                         if (bad >> e & 1u) x = __builtin_nanf("");
-                        if (page[u] < 0 || t0 + e < vis.lo || t0 + e >= vis.hi) x = kNone;
+                        if (page[su] < 0 || t0 + e < vis.lo || t0 + e >= vis.hi) x = kNone;
                         sc[u][e] = x;
                         top = __builtin_fmaxf(top, x);
                     }
                 }
-            } else {
+                follow(other_half_max(top));
+                const float base = m == kNone ? 0.f : m;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float x = sc[u][0];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[u][e]);
-                    top = __builtin_fmaxf(top, __builtin_fmaf(x, ks[u], vsc[u].log));  // ks >= 0: the largest product is the largest score
-                }
+                for (int u = 0; u < 2; ++u) powers(u, 1.f, -(base - lift), vsc[ONE ? 0 : u].factor);
+                outputs(0);
+                outputs(1);
             }
-            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-            const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
-            m = top;
-            l *= alpha;
-            u32x4 p[2][2][PP];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                // the scores are there already (mul 1, add 0) or still to be made from the products
-                const float mul = odd ? 1.f : ks[u], add = (odd ? 0.f : vsc[u].log) - (base - kLift);
-                float sum = 0.f;
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * v + e], mul, add));
-                        sum += x[e];
-                    }
-                    if (odd)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] *= vsc[u].factor;
-                    split_parts<_Float16, PP>(x, p[u][v]);
-                }
-                l = __builtin_fmaf(sum, vsc[u].inv, l);
-            }
-            if (__any(alpha != 1.f)) {
-#pragma unroll
-                for (int t = 0; t < DT; ++t) o[t] *= alpha;
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) {
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(vl + vrow + t * 32 * VPITCH + u * 64 + v * 16);
-#pragma unroll
-                        for (int k = 0; k < PP; ++k) o[t] = mma32<_Float16>(x, p[u][v][k], o[t]);
-                    }
         }
-        __syncthreads();
+        __syncthreads();  // and is left by everybody
     }
     l += __shfl_xor(l, 32);
     if (!real) return;
@@ -682,7 +765,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
                 const int d = t * 32 + b * 8 + h2 * 4;
                 if (d < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + d) = f32x4_t{o[t][4 * b], o[t][4 * b + 1], o[t][4 * b + 2], o[t][4 * b + 3]};
             }
-        if (h2 == 0) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+        if (h2 == 0) { a.part_ml[2 * slot] = m - lift; a.part_ml[2 * slot + 1] = l; }
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -694,7 +777,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
             const int d = t * 32 + b * 8 + h2 * 4;
             if (d < D) store4<T>(dst + d, o[t][4 * b] * inv, o[t][4 * b + 1] * inv, o[t][4 * b + 2] * inv, o[t][4 * b + 3] * inv);
         }
-    if (h2 == 0 && a.lse) a.lse[at] = lse_of(m, l);
+    if (h2 == 0 && a.lse) a.lse[at] = lse_of(m - lift, l);
 }
 
 // ---- the slices of a row ------------------------------------------------------------------------------------------------
@@ -752,8 +835,14 @@ static __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const A
 constexpr int kWaves = 4, kTileRows = kWaves * 32;
 template <typename T, typename Code, int SPANS, bool EXACT, bool ONE> void launch_one(const AttArgs &a, hipStream_t st) {
     const unsigned blocks = (unsigned)((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits);
-    if (a.tile_rows == 16) kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE><<<blocks, kBlock, 0, st>>>(a);
-    else kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+    if (a.tile_rows == 16) {
+        if constexpr (ONE) {
+            if (a.nt) { kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, true><<<blocks, kBlock, 0, st>>>(a); return; }
+        }
+        kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, false><<<blocks, kBlock, 0, st>>>(a);
+    } else {
+        kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+    }
 }
 // head sizes that fill their registers need no bounds in the loops, pages of at least 64 tokens no page number a lane
 template <typename T, typename Code, int SPANS> void launch_dim(const AttArgs &a, hipStream_t st) {

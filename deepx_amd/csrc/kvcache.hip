@@ -231,7 +231,6 @@ __global__ __launch_bounds__(THREADS) void kvcache_read_kernel(const RowsArgs a)
     constexpr int V = kVecBytes / (int)sizeof(T);
     const int per_row = D / V;
     if (which == 0) {
-#pragma unroll 2
         for (int i = threadIdx.x + t0 * per_row; i < t1 * per_row; i += THREADS) {  // V codes into 16 bytes of a row
             const int t = i / per_row, d = (i - t * per_row) * V;
             float y[V];

@@ -157,8 +157,9 @@ def attention_bar(name, c, entry):
       products with scales: (D/32 + 40) u of scale sum|q||k|; f32 rows add 2^-24 of it for the split of q.
       probability: that as a relative error, the rounding of s - m (2 u |s - m|, |s - m| under twice the largest score) and of 2^x (4 u).
       sums over N tokens: (N/32 + 64) u.  Both the sum and its normalisation carry these: twice.
-      rounding of p * v_scale to f16, or to two f16 parts for f32 rows: 2^-11, 2^-22 of sum p|v|; p * v_scale is held relative to its largest, 2^15
-      times as large, so that f16's smallest steps add at most 2^-25 2^-15 of the largest times a code for each token; of the result: half a step.
+      rounding of p * v_scale to f16, or to two f16 parts for f32 rows: 2^-11, 2^-22 of sum p|v|; p * v_scale is held relative to its largest, at least
+      2^7 times as large for f16 and bf16 rows and 2^15 times for f32 rows, so that f16's smallest steps (half of 2^-24) add at most 2^-32, 2^-40 of
+      the largest times a code for each token; of the result: half a step.
       underflow: the hardware's 2^x gives 0 below 2^-126, the smallest normal fp32 number; with l >= 1 (the largest term is 1) each of the N
       terms is off by at most 2^-126 max|v|."""
     out, lse, mag, big, n, top, weight = entry
@@ -166,5 +167,5 @@ def attention_bar(name, c, entry):
     s = ((c.dim / 32 + 42) * big + 4 * big + 4) * u
     sums = (n / 32 + 64) * u
     part = {"bf16": 2.0 ** -11, "f16": 2.0 ** -11, "f32": 2.0 ** -22}[name]
-    bar = (n * 2.0 ** -40 * float(MAX[c.code]) * weight)[:, None] + mag * (part + 2 * s + 2 * sums)[:, None] + np.abs(out) * HALF_STEP[name] * (1 + 2 ** -8) + TINY[name] + n * 2.0 ** -126 * top
+    bar = (n * (2.0 ** -40 if name == "f32" else 2.0 ** -32) * float(MAX[c.code]) * weight)[:, None] + mag * (part + 2 * s + 2 * sums)[:, None] + np.abs(out) * HALF_STEP[name] * (1 + 2 ** -8) + TINY[name] + n * 2.0 ** -126 * top
     return bar, s + sums + np.abs(np.where(np.isfinite(lse), lse, 0)) * 2 * u

@@ -156,8 +156,8 @@ __device__ __forceinline__ void reach(ValueScale &v, float largest) {
 // The tokens [lo, hi) that row i of a sequence sees; nothing for a row that is none or has no place in the cache.
 struct Range { int lo, hi; };
 __device__ __forceinline__ Range row_range(const AttArgs &a, const KvSeq &s, int i) {
+    if (i >= s.n || s.begin + i < 0) return {0, 0};
     const int p = s.begin + i;
-    if (i >= s.n || p < 0) return {0, 0};
     const int hi = a.causal && p + 1 < s.length ? p + 1 : s.length;
     const int lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
     return {lo < hi ? lo : hi, hi};
@@ -223,15 +223,15 @@ template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, f
 __device__ __forceinline__ float lse_of(float ref, float l) { return l == 0.f ? kNone : kLn2 * (ref + __builtin_amdgcn_logf(l)); }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
-// One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its four waves take every fourth 64-token tile
-// and meet at the end.  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
+// One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its waves take the 64-token tiles in
+// turn and meet at the end (four waves; eight where there is at most a workgroup a CU: one row over 777 tokens 9.0 -> 8.4 us).  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
 // loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes.
-template <typename T, typename Code, int SPANS, bool EXACT, bool ONE, bool NT>
-static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
+template <typename T, typename Code, int SPANS, bool EXACT, bool ONE, bool NT, int WAVES>
+static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
-    __shared__ float meet_o[2][16][SPANS * 64 + 4];
-    __shared__ float meet_m[4][16], meet_l[4][16];
+    __shared__ float meet_o[WAVES / 2][16][SPANS * 64 + 4];
+    __shared__ float meet_m[WAVES][16], meet_l[WAVES][16];
     unsigned blk = blockIdx.x;
     const int split = blk % (unsigned)a.splits; blk /= (unsigned)a.splits;
     const int rt = blk % (unsigned)a.row_tiles; blk /= (unsigned)a.row_tiles;
@@ -289,7 +289,7 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
         entries(tile);
         load_keys(tile);
         load_values(tile, gp);
-        entries(tile + 4);
+        entries(tile + WAVES);
     }
 
     // this lane's row
@@ -315,7 +315,7 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (; tile < tile_end; tile += 4) {
+    for (; tile < tile_end; tile += WAVES) {
         const int tok0 = tile * 64, gb = tok0 + gofs;
         ValueScale vsc = value_scale(vs);
         {
@@ -327,7 +327,7 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
             largest = __builtin_fmaxf(largest, x);
             reach(vsc, largest);
         }
-        const bool none = gp < 0, fine = finite(vs), more = tile + 4 < tile_end;
+        const bool none = gp < 0, fine = finite(vs), more = tile + WAVES < tile_end;
         const float mul = ks * a.scale;
         const bool odd = tok0 < all_lo || tok0 + 64 > all_hi || __any(none || !fine);
         float sc[16];
@@ -344,7 +344,7 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
             for (int e = 0; e < 4; ++e) sc[4 * t + e] = __builtin_fmaf(acc[e], mul, vsc.log);
         }
         // the keys' registers are free: the next tile's keys come while this one's values are used
-        if (more) load_keys(tile + 4);
+        if (more) load_keys(tile + WAVES);
         if (odd) {
             uint32_t bad = fine ? 0u : 0xffffu;  // bit j: the score of token 16 g + j becomes NaN
             if constexpr (std::is_same_v<Code, CodeE4M3>) {
@@ -401,26 +401,26 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
             }
         }
         if (more) {
-            load_values(tile + 4, gp);
-            entries(tile + 8);
+            load_values(tile + WAVES, gp);
+            entries(tile + 2 * WAVES);
         }
     }
 
-    // the four waves meet: l over the lane groups, then everything relative to the common maximum, added in wave order
+    // the waves meet: l over the lane groups, then everything relative to the common maximum, added in wave order
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g == 0) meet_m[wave][n] = m;
     __syncthreads();
     float top = meet_m[0][n];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = __builtin_fmaxf(top, meet_m[w][n]);
+    for (int w = 1; w < WAVES; ++w) top = __builtin_fmaxf(top, meet_m[w][n]);
     const float base = top == kNone ? 0.f : top, mine = __builtin_amdgcn_exp2f(m - base);
     l *= mine;
     if (g == 0) meet_l[wave][n] = l;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] *= mine;
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {  // waves 2, 3 give to 0, 1; then 1 to 0
+    for (int half = WAVES / 2; half >= 1; half >>= 1) {  // the upper half of the waves gives to the lower, until one is left
         if (wave >= half && wave < 2 * half)
 #pragma unroll
             for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t *>(&meet_o[wave - half][n][t * 16 + g * 4]) = o[t];
@@ -431,7 +431,9 @@ static __global__ __launch_bounds__(kBlock, SPANS == 4 ? 1 : SPANS == 2 || RowTy
         __syncthreads();
     }
     if (wave != 0 || !real) return;
-    l = (meet_l[0][n] + meet_l[1][n]) + (meet_l[2][n] + meet_l[3][n]);
+    l = meet_l[0][n];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) l += meet_l[w][n];
     const int64_t at = (s.first + i) * a.q_heads + h;
     if (a.splits > 1) {
         const int64_t slot = (int64_t)split * a.kv.rows * a.q_heads + at;
@@ -837,9 +839,12 @@ template <typename T, typename Code, int SPANS, bool EXACT, bool ONE> void launc
     const unsigned blocks = (unsigned)((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits);
     if (a.tile_rows == 16) {
         if constexpr (ONE) {
-            if (a.nt) { kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, true><<<blocks, kBlock, 0, st>>>(a); return; }
+            if (a.nt) { kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, true, 4><<<blocks, kBlock, 0, st>>>(a); return; }
         }
-        kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, false><<<blocks, kBlock, 0, st>>>(a);
+        if constexpr (SPANS <= 2) {
+            if (blocks <= (unsigned)kCUs) { kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, false, 8><<<blocks, 8 * kWave, 0, st>>>(a); return; }
+        }
+        kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, false, 4><<<blocks, kBlock, 0, st>>>(a);
     } else {
         kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
     }

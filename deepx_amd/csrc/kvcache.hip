@@ -171,7 +171,10 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
     const int64_t start = (int64_t)slot * P;  // first token of the page; new ones are t0 .. t1 - 1 of it, older ones 0 .. t0 - 1
     const int t0 = (int)(s.begin > start ? s.begin - start : 0), t1 = (int)((int64_t)s.begin + s.n - start < P ? (int64_t)s.begin + s.n - start : P);
     if (t1 <= t0) return;
-    const int64_t page = kv_page(a.kv, seq, slot);  // not looked at before the rows are on their way
+    // the table's entry comes beside the rows; only their codes need to know the page
+    const int64_t entry_at = (int64_t)seq * a.kv.pages_per_seq + (slot < 0 ? 0 : slot < a.kv.pages_per_seq ? slot : a.kv.pages_per_seq - 1);
+    const bool has_slot = slot >= 0 && slot < a.kv.pages_per_seq;
+    const int64_t entry = !a.kv.table ? entry_at : a.kv.pages_per_seq > 0 ? (int64_t)a.kv.table[entry_at] : -1;
     const T *x = (const T *)a.data[which] + (s.first + (start + t0 - s.begin)) * a.row_stride[which] + head * a.head_stride[which];
     const int64_t pitch = a.row_stride[which];
 
@@ -198,6 +201,7 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
         }
         top = __builtin_fminf(bits_to_float(block_max<THREADS>(float_to_bits(y))), 3.4028234663852886e38f);
     }
+    const int64_t page = has_slot && entry >= 0 && entry < a.kv.num_pages ? entry : -1;
     if (page < 0) return;  // the same for the whole workgroup
     const int64_t where = page * a.kv.heads + head;
     float *scale_at = (which ? a.kv.v_scale : a.kv.k_scale) + where;
@@ -277,8 +281,8 @@ __global__ __launch_bounds__(THREADS) void kvcache_read_kernel(const RowsArgs a)
 template <typename T, typename Code> int launch(const RowsArgs &a, bool write, hipStream_t st) {
     const int64_t blocks = (int64_t)2 * a.kv.heads * a.slots * a.kv.batch;
     if (blocks > INT32_MAX) return DXH_ERR_TOO_LARGE;
-    // a wave is enough for the pieces of a few rows; a whole page of them goes to four
-    const bool wide = std::min(a.kv.max_rows, a.kv.page_size) * a.kv.dim > 2048;
+    // a lane for every 16 codes of a page, as one new row can change the scale of all: one wave or four
+    const bool wide = a.kv.page_size * a.kv.dim > 16 * kWave;
     if (write) {
         if (wide) kvcache_write_kernel<T, Code, 256><<<(unsigned)blocks, 256, 0, st>>>(a);
         else kvcache_write_kernel<T, Code, 64><<<(unsigned)blocks, 64, 0, st>>>(a);

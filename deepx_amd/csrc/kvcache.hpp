@@ -88,7 +88,8 @@ inline int kv_check(const dxh_kvcache *c, const dxh_kvrows *r, int dtype, KvArgs
     if (c->dim < 16 || c->dim > 256 || c->dim % 16) return DXH_ERR_SHAPE;
     if (!c->page_table && c->num_pages < (int64_t)r->batch * c->pages_per_seq) return DXH_ERR_SHAPE;
     if (!r->offsets && r->rows < (int64_t)r->batch * r->max_rows) return DXH_ERR_SHAPE;
-    if (r->rows > INT32_MAX || c->num_pages > INT32_MAX) return DXH_ERR_TOO_LARGE;
+    // tokens are counted in 32 bits, a few tiles past the last one included
+    if (r->rows > INT32_MAX || c->num_pages > INT32_MAX || (int64_t)c->pages_per_seq * c->page_size > ((int64_t)1 << 30)) return DXH_ERR_TOO_LARGE;
     if (!aligned(c->k, kVecBytes) || !aligned(c->v, kVecBytes) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(c->page_table, 4) ||
         !aligned(r->offsets, 4) || !aligned(r->lengths, 4)) return DXH_ERR_ALIGN;
     a = KvArgs{};

@@ -532,7 +532,8 @@ DXH_API int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int
  *   page_table        [batch, pages_per_seq] int32: the page that holds tokens i * page_size ... of sequence b; NULL: page
  *                     b * pages_per_seq + i (a cache without paging).  An entry outside [0, num_pages) is no page: nothing
  *                     is written there, reads give zeros, the attention sees no tokens in it.
- * code: DXH_I8 or DXH_F8E4M3.  page_size 16, 32, 64 or 128; dim a multiple of 16 up to 256; k and v 16-byte aligned.
+ * code: DXH_I8 or DXH_F8E4M3.  page_size 16, 32, 64 or 128; at most 2^30 tokens a sequence; dim a multiple of 16 up to 256;
+ * k and v 16-byte aligned.
  *
  * The rows of a call are packed [rows, heads, dim]: sequence b has the rows offsets[b] .. offsets[b + 1] - 1 (device int32
  * [batch + 1], ascending), and they are the last of the lengths[b] tokens (device int32 [batch]) that the sequence holds in
@@ -576,8 +577,9 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * pages without visible tokens included; a NaN among a visible token's values makes that dimension of the row, or the whole
  * row, NaN, and so does a scale of a visible token's page that is not finite.  dtype f32 f16 bf16 for q and out (which must
  * not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
- * queries enter the products exactly; a probability is rounded to f16, held relative to the largest, for f16 and bf16 rows and
- * kept to 22 bits for f32 rows.
+ * queries enter the products exactly; a probability, together with its value scale, is rounded to f16, held relative to the
+ * largest, for f16 and bf16 rows and kept to 22 bits for f32 rows (values whose page's scale is below 2^-85 of the largest scale
+ * met may count as zeros).
  * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a
  * second launch: device memory of the caller of at least the query's bytes, 256-byte aligned, that no other call in flight
  * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows and q_heads alone; workspace may be NULL when it is 0. */

@@ -92,7 +92,8 @@ def kvrows(**kw):
 
 BAD_CACHE = [(dict(code=dx.I16), DTYPE), (dict(code=dx.BF16), DTYPE), (dict(num_pages=-1), ARG), (dict(pages_per_seq=-1), ARG), (dict(heads=0), ARG), (dict(page_size=8), SHAPE),
              (dict(page_size=48), SHAPE), (dict(page_size=256), SHAPE), (dict(dim=24), SHAPE), (dict(dim=272), SHAPE), (dict(dim=0), SHAPE), (dict(k=4100), ALIGN), (dict(v=8193), ALIGN),
-             (dict(k_scale=258), ALIGN), (dict(page_table=1026), ALIGN), (dict(page_table=None, num_pages=31), SHAPE)]
+             (dict(k_scale=258), ALIGN), (dict(page_table=1026), ALIGN), (dict(page_table=None, num_pages=31), SHAPE),
+             (dict(pages_per_seq=(1 << 26) + 1), -6), (dict(num_pages=1 << 31), -6)]
 BAD_ROWS = [(dict(batch=-1), ARG), (dict(rows=-1), ARG), (dict(max_rows=-1), ARG), (dict(offsets=258), ALIGN), (dict(lengths=514), ALIGN), (dict(offsets=None, rows=31), SHAPE),
             (dict(rows=1 << 31), -6), (dict(rows=1, lengths=None), ARG)]
 

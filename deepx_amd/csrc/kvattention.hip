@@ -8,12 +8,20 @@ namespace {
 constexpr int64_t kFewRows = 32;  // rows of one sequence and key head up to which the 16-row kernel runs
 
 // How many slices the tokens of a sequence are cut into, counted on the longest sequence that the cache can hold; a slice has at
-// least kMinTiles tiles (slice_tiles), so that short sequences use fewer.  The sequences of a batch differ in length: 8
-// workgroups a CU let the card fill the gaps that short ones leave (64 sequences of 1k-16k tokens: 245 us at 4, 229 at 8, 230
-// at 16); one sequence is cut into what runs at once, two workgroups a CU (131071 tokens: 64 us at 2, 76 at 4).
-int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few) {
+// least min_tiles tiles (slice_tiles), so that short sequences use fewer.
+//   Few rows (16 tiles a slice): the sequences of a batch differ in length, and 8 workgroups a CU let the card fill the gaps that
+//   short ones leave (64 sequences of 1k-16k tokens: 245 us at 4, 229 at 8, 230 at 16); one sequence is cut into what runs at once,
+//   two workgroups a CU (131071 tokens: 64 us at 2, 76 at 4).  16 against 8 tiles a slice: one row over 777 tokens, one launch
+//   instead of two, 9.3 and 11.6 us.
+//   Many rows (4 tiles; 16 for heads over 128, whose partial results are twice as long: eight prompts of 313-364 tokens, 8 heads of
+//   256, 57 us uncut and 67 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
+//   7 / 1 heads of 64: 82 us uncut, 39 in slices).
+int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few, int min_tiles) {
     const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles, tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
-    int64_t want = std::min<int64_t>(((few && kv.batch > 1 ? 8 : 2) * kCUs + blocks - 1) / blocks, (tiles + kMinTiles - 1) / kMinTiles);
+    int64_t want;
+    if (few) want = ((kv.batch > 1 ? 8 : 2) * kCUs + blocks - 1) / blocks;
+    else want = blocks < 2 * kCUs ? (4 * kCUs + blocks - 1) / blocks : 1;
+    want = std::min<int64_t>(want, (tiles + min_tiles - 1) / min_tiles);
     const int64_t row_bytes = kv.rows * q_heads * (kv.dim + 2) * 4;
     want = std::min<int64_t>(want, ((int64_t)256 << 20) / std::max<int64_t>(1, row_bytes));  // partial results of at most 256 MiB
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
@@ -36,7 +44,8 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     if (most > INT32_MAX - kTileRows) return DXH_ERR_TOO_LARGE;
     a.tile_rows = most <= kFewRows ? 16 : kTileRows;
     a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
-    a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16);
+    a.min_tiles = a.tile_rows == 16 || a.kv.dim > 128 ? 16 : 4;
+    a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16, a.min_tiles);
     if ((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits > INT32_MAX || (int64_t)a.kv.batch * a.kv.max_rows * q_heads > INT32_MAX) return DXH_ERR_TOO_LARGE;
     return DXH_OK;
 }

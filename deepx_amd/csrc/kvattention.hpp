@@ -33,7 +33,7 @@ struct AttArgs {
     int64_t q_row, q_head, o_row, o_head;
     float *lse, *part_o, *part_ml;  // partials: [slice][packed row][q head][dim] and [slice][packed row][q head][2]
     float scale;                    // scale * log2(e)
-    int q_heads, group, causal, window, splits, row_tiles, tile_rows;
+    int q_heads, group, causal, window, splits, min_tiles, row_tiles, tile_rows;
     int nt;  // few rows and pages of at least 64 tokens: the codes are read past the last-level cache
 };
 
@@ -173,15 +173,14 @@ __device__ __forceinline__ void tile_range(const AttArgs &a, const KvSeq &s, int
     first = x.lo / 64;
     last = (y.hi + 63) / 64;
 }
-// tiles in a slice when `tiles` of them are cut into at most `splits` slices: no fewer than kMinTiles
-constexpr int kMinTiles = 16;
-__device__ __forceinline__ int slice_tiles(int tiles, int splits) {
-    const int each = (tiles + splits - 1) / splits;
-    return each < kMinTiles ? kMinTiles : each;
+// tiles in a slice when `tiles` of them are cut into at most a.splits slices: no fewer than a.min_tiles
+__device__ __forceinline__ int slice_tiles(const AttArgs &a, int tiles) {
+    const int each = (tiles + a.splits - 1) / a.splits;
+    return each < a.min_tiles ? a.min_tiles : each;
 }
 // the part of [first, last) that slice `split` walks; false if there is none (slice 0 always has one, if empty)
 __device__ __forceinline__ bool slice_of(const AttArgs &a, int split, int &first, int &last) {
-    const int each = a.splits > 1 ? slice_tiles(last - first, a.splits) : last - first, b = first + split * each;
+    const int each = a.splits > 1 ? slice_tiles(a, last - first) : last - first, b = first + split * each;
     last = b + each < last ? b + each : last;
     first = b;
     return split == 0 || first < last;
@@ -783,54 +782,51 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
 }
 
 // ---- the slices of a row ------------------------------------------------------------------------------------------------
-// One workgroup for a packed row and query head.  Groups of dim / 4 lanes (rounded up to a power of two) take every so many-th
-// slice, each in one pass with a running maximum, and meet in LDS; the group's sums are added in group order.
+// Groups of dim / 4 lanes (rounded up to a power of two) add the slices of a packed row and query head, each in one pass with a
+// running maximum.  Up to kFewSlices one group takes all slices of its own row; beyond, the groups of a workgroup share one
+// row, every group every so many-th slice, and meet in LDS, where the sums are added in group order.
+constexpr int kFewSlices = 16;
+struct Joined { float m, l; f32x4_t o; };
+__device__ __forceinline__ void join_one(Joined &j, float m, float l, const f32x4_t &o) {
+    const float top = __builtin_fmaxf(j.m, m), base = top == kNone ? 0.f : top;
+    const float wa = __builtin_amdgcn_exp2f(j.m - base), wb = __builtin_amdgcn_exp2f(m - base);
+    j.o = j.o * wa + o * wb;
+    j.l = __builtin_fmaf(j.l, wa, l * wb);
+    j.m = top;
+}
 template <typename T>
 static __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs a) {
     __shared__ f32x4_t meet_o[kBlock];
     __shared__ float meet_m[16], meet_l[16];
-    unsigned blk = blockIdx.x;
+    const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64, groups = kBlock / lanes, group = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
+    const bool shared = a.splits > kFewSlices, live = d < a.kv.dim;
+    unsigned blk = shared ? blockIdx.x : blockIdx.x * groups + group;
     const int h = blk % (unsigned)a.q_heads; blk /= (unsigned)a.q_heads;
     const int i = blk % (unsigned)a.kv.max_rows, seq = blk / (unsigned)a.kv.max_rows;
+    if (seq >= a.kv.batch) return;  // whole groups; in the shared form the grid is exact
     const KvSeq s = kv_seq(a.kv, seq);
     if (i >= s.n) return;
     const int r0 = (i * a.group + h % a.group) / a.tile_rows * a.tile_rows;
     int first, last;
     tile_range(a, s, r0 / a.group, (r0 + a.tile_rows - 1) / a.group, first, last);
-    const int each = slice_tiles(last - first, a.splits), used = last > first ? (last - first + each - 1) / each : 1;
+    const int each = slice_tiles(a, last - first), used = last > first ? (last - first + each - 1) / each : 1;
     const int64_t at = (s.first + i) * a.q_heads + h, pitch = a.kv.rows * a.q_heads;
-    const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64, groups = kBlock / lanes, group = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
-    const bool live = d < a.kv.dim;
     const float *po = a.part_o + at * a.kv.dim + (live ? d : 0), *pm = a.part_ml + 2 * at;
-    float m = kNone, l = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    Joined j{kNone, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    const int step = shared ? groups : 1;
 #pragma unroll 4
-    for (int k = group; k < used; k += groups) {
-        const f32x4_t x = *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim);
-        const float mk = pm[2 * k * pitch], lk = pm[2 * k * pitch + 1];
-        const float top = __builtin_fmaxf(m, mk), base = top == kNone ? 0.f : top;
-        const float wa = __builtin_amdgcn_exp2f(m - base), wb = __builtin_amdgcn_exp2f(mk - base);
-        o = o * wa + x * wb;
-        l = __builtin_fmaf(l, wa, lk * wb);
-        m = top;
+    for (int k = shared ? group : 0; k < used; k += step)
+        join_one(j, pm[2 * k * pitch], pm[2 * k * pitch + 1], *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim));
+    if (shared) {  // the same for the whole workgroup
+        meet_o[threadIdx.x] = j.o;
+        if (d == 0) { meet_m[group] = j.m; meet_l[group] = j.l; }
+        __syncthreads();
+        if (group > 0) return;
+        for (int k = 1; k < groups; ++k) join_one(j, meet_m[k], meet_l[k], meet_o[k * lanes + threadIdx.x]);
     }
-    meet_o[threadIdx.x] = o;
-    if (threadIdx.x % lanes == 0) { meet_m[group] = m; meet_l[group] = l; }
-    __syncthreads();
-    if (group > 0) return;
-    float top = m;
-    for (int k = 1; k < groups; ++k) top = __builtin_fmaxf(top, meet_m[k]);
-    const float base = top == kNone ? 0.f : top;
-    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    l = 0.f;
-    for (int k = 0; k < groups; ++k) {
-        const float w = __builtin_amdgcn_exp2f(meet_m[k] - base);
-        o += meet_o[k * lanes + threadIdx.x] * w;
-        l = __builtin_fmaf(meet_l[k], w, l);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (threadIdx.x == 0 && a.lse) a.lse[at] = lse_of(top, l);
+    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, j.o[0] * inv, j.o[1] * inv, j.o[2] * inv, j.o[3] * inv);
+    if (d == 0 && a.lse) a.lse[at] = lse_of(j.m, j.l);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
@@ -861,7 +857,8 @@ template <typename T, typename Code> int kvattention_launch(const AttArgs &a, hi
     else launch_dim<T, Code, 4>(a, st);
     const int rc = launch_status();
     if (rc != DXH_OK || a.splits == 1) return rc;
-    kvattention_join_kernel<T><<<(unsigned)((int64_t)a.kv.batch * a.kv.max_rows * a.q_heads), kBlock, 0, st>>>(a);
+    const int64_t rows = (int64_t)a.kv.batch * a.kv.max_rows * a.q_heads, at_once = a.splits > kFewSlices ? 1 : kBlock / (a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64);
+    kvattention_join_kernel<T><<<(unsigned)((rows + at_once - 1) / at_once), kBlock, 0, st>>>(a);
     return launch_status();
 }
 

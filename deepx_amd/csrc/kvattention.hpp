@@ -5,7 +5,7 @@
 //     s_j = (Q K'^T)_j k_s(j) scale log2(e),     t_j = s_j + log2 v_s(j),     m = max t_j,     p_j = 2^(t_j - m),
 //     O   = sum p_j V'_j,     l = sum p_j / v_s(j),     out = O / l,     lse = ln 2 (m + log2 l).
 // Taking the value scale into the exponent keeps p in (0, 1] whatever the scales are, so that it can be rounded to f16 (held
-// 2^15 times as large: normal down to 2^-29 of the largest): 2^-11 of a term where bf16 would lose 2^-8, on the same matrix
+// 2^15 times as large, or 2^7 times with 128-row tiles: normal down to 2^-29 or 2^-21 of the largest): 2^-11 of a term where bf16 would lose 2^-8, on the same matrix
 // instruction.  Codes are whole numbers below 2^8 or e4m3 values, exact in bf16 and in f16, and enter the products
 // exactly; scales are applied to scores in fp32.  Q is exact too: bf16 rows multiply bf16 keys, f16 rows f16 keys; f32 rows are split
 // into three bf16 parts (24 bits) and their p into two f16 parts, each part one more product.
@@ -44,7 +44,9 @@ constexpr float kLift = 15.f;        // probabilities are held 2^15 times as lar
 // kSlack (in powers of two): the output is then rescaled in few tiles, and a probability, held 2^(15 - kSlack) times as large, is
 // still at most 2^15.
 constexpr float kSlack = 8.f;
-constexpr float kTinyScale = 0x1p-100f;  // value scales below it are multiplied into the codes: 1 / scale stays finite
+// A row's sum of (2^15 times) p / v_scale, kept 2^-9 times as large, is finite for 2^30 tokens of the smallest scale, 2^-92 (what is
+// below is multiplied into the probabilities), and no less than 2^-123 for one token of the largest that fp32 values get, 2^121.
+constexpr float kTinyScale = 0x1p-92f, kSumUnit = 0x1p-9f, kSumLog = 9.f;
 
 // ---- products ---------------------------------------------------------------------------------------------------------
 // Kind: the 16-bit type of keys and queries; QP, PP: parts that hold a query value, a probability
@@ -138,9 +140,9 @@ struct ValueScale { float log, inv, factor; };
 __device__ __forceinline__ ValueScale value_scale(float vs) {
     if (!finite(vs)) vs = 1.f;
     const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
-    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p100f};
+    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p92f};
 }
-// Where a scale is so much smaller than the largest so far that 2^(t - m) could be 0 while the token's share of l is not (a page of
+// Where a scale is so much smaller than the largest that the row has seen so far that 2^(t - m) could be 0 while the token's share of l is not (a page of
 // zeros beside one of huge values), the exponent keeps within kReach of that largest one's and the rest of the scale becomes a
 // factor.  What it is a factor of is then below 2^-85 of the largest values.
 constexpr float kReach = 85.f;
@@ -151,6 +153,14 @@ __device__ __forceinline__ void reach(ValueScale &v, float largest) {
     v.inv = __builtin_amdgcn_exp2f(kReach - largest);
     v.log = largest - kReach;
 }
+// 2^x, x <= 0, for a row whose reference moves.  Its sum holds 1 / scale of every token and may count although 2^x is less than any
+// float (tokens of scale 2^-92 beside some of 2^60 that weigh the same): it is multiplied by 2^(x / 2) twice.
+struct Shift {
+    float half;
+    __device__ __forceinline__ float all() const { return half * half; }
+    __device__ __forceinline__ float sum(float l) const { return l * half * half; }
+};
+__device__ __forceinline__ Shift shift_of(float x) { return {__builtin_amdgcn_exp2f(0.5f * x)}; }
 
 // ---- which tokens -------------------------------------------------------------------------------------------------------
 // The tokens [lo, hi) that row i of a sequence sees; nothing for a row that is none or has no place in the cache.
@@ -162,6 +172,7 @@ __device__ __forceinline__ Range row_range(const AttArgs &a, const KvSeq &s, int
     const int lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
     return {lo < hi ? lo : hi, hi};
 }
+__device__ __forceinline__ bool sees(const Range &r, int token, int n) { return token < r.hi && token + n > r.lo; }  // any of n tokens
 // 64-token tiles that rows i0 .. i1 of a sequence see between them: [first, last)
 __device__ __forceinline__ void tile_range(const AttArgs &a, const KvSeq &s, int i0, int i1, int &first, int &last) {
     if (i1 >= s.n) i1 = s.n - 1;
@@ -218,8 +229,8 @@ template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, f
     store_acc_vec<T, 4>(w, y);
     *reinterpret_cast<vec_t<T, 4> *>(dst) = w;
 }
-// `ref`: the power of two that l (and the output) are counted in
-__device__ __forceinline__ float lse_of(float ref, float l) { return l == 0.f ? kNone : kLn2 * (ref + __builtin_amdgcn_logf(l)); }
+// `ref`: the power of two that l / kSumUnit and the output are counted in
+__device__ __forceinline__ float lse_of(float ref, float l) { return l == 0.f ? kNone : kLn2 * (ref + kSumLog + __builtin_amdgcn_logf(l)); }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
 // One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its waves take the 64-token tiles in
@@ -309,7 +320,7 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
     const int last_row = (r0 + 15 < rows ? r0 + 15 : rows - 1) / G;
     const int all_lo = row_range(a, s, last_row).lo, all_hi = row_range(a, s, r0 / G).hi;
 
-    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale
+    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale that the row has seen
     f32x4_t o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -317,8 +328,9 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
     for (; tile < tile_end; tile += WAVES) {
         const int tok0 = tile * 64, gb = tok0 + gofs;
         ValueScale vsc = value_scale(vs);
+        const bool cut = tok0 < all_lo || tok0 + 64 > all_hi;
         {
-            float x = gp < 0 ? kNone : vsc.log;
+            float x = gp < 0 || (cut && !sees(vis, ONE ? tok0 : gb, ONE ? 64 : 16)) ? kNone : vsc.log;
             if constexpr (!ONE) {
                 x = __builtin_fmaxf(x, __shfl_xor(x, 16));
                 x = __builtin_fmaxf(x, __shfl_xor(x, 32));
@@ -328,7 +340,7 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
         }
         const bool none = gp < 0, fine = finite(vs), more = tile + WAVES < tile_end;
         const float mul = ks * a.scale;
-        const bool odd = tok0 < all_lo || tok0 + 64 > all_hi || __any(none || !fine);
+        const bool odd = cut || __any(none || !fine);
         float sc[16];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -373,7 +385,8 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
         for (int e = 0; e < 16; ++e) top = __builtin_fmaxf(top, sc[e]);
         top = __builtin_fmaxf(top, __shfl_xor(top, 16));
         top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == kNone ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - base);
+        const float base = top == kNone ? 0.f : top;
+        const Shift shift = shift_of(m - base);
         m = top;
         float sum = 0.f;
         u32x4 p[2][PP];
@@ -388,10 +401,10 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
             }
             split_parts<_Float16, PP>(x, p[u]);
         }
-        l = __builtin_fmaf(sum, vsc.inv, l * alpha);
+        l = __builtin_fmaf(sum * kSumUnit, vsc.inv, shift.sum(l));
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            o[t] *= alpha;
+            o[t] *= shift.all();
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const u32x4 v = codes8<Code, _Float16>(vc[t][2 * u], vc[t][2 * u + 1]);
@@ -413,11 +426,11 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
     float top = meet_m[0][n];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) top = __builtin_fmaxf(top, meet_m[w][n]);
-    const float base = top == kNone ? 0.f : top, mine = __builtin_amdgcn_exp2f(m - base);
-    l *= mine;
+    const Shift mine = shift_of(m - (top == kNone ? 0.f : top));
+    l = mine.sum(l);
     if (g == 0) meet_l[wave][n] = l;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] *= mine;
+    for (int t = 0; t < DT; ++t) o[t] *= mine.all();
 #pragma unroll
     for (int half = WAVES / 2; half >= 1; half >>= 1) {  // the upper half of the waves gives to the lower, until one is left
         if (wave >= half && wave < 2 * half)
@@ -442,7 +455,7 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
         if (g == 0) { a.part_ml[2 * slot] = top - kLift; a.part_ml[2 * slot + 1] = l; }
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : kSumUnit / l;
     T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -531,7 +544,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
         }
     }
 
-    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale
+    float m = kNone, l = 0.f, largest = kNone;  // largest: logarithm of a value scale that the row has seen
     f32x16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -648,8 +661,15 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
 #pragma unroll
         for (int u = 0; u < S; ++u) vsc[u] = value_scale(vs[u]);
         {
-            float x = page[0] < 0 ? kNone : vsc[0].log;
-            if constexpr (!ONE) x = other_half_max(__builtin_fmaxf(x, page[S - 1] < 0 ? kNone : vsc[S - 1].log));
+            float y[S];
+#pragma unroll
+            for (int u = 0; u < S; ++u) y[u] = page[u] < 0 ? kNone : vsc[u].log;
+            if (cut) {
+#pragma unroll
+                for (int u = 0; u < S; ++u) y[u] = sees(vis, ONE ? tok0 : tok0 + u * 32 + h2 * 16, ONE ? 64 : 16) ? y[u] : kNone;
+            }
+            float x = __builtin_fmaxf(y[0], y[S - 1]);
+            if constexpr (!ONE) x = other_half_max(x);
             largest = __builtin_fmaxf(largest, x);
         }
 #pragma unroll
@@ -685,7 +705,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
                 }
                 split_parts<_Float16, PP>(x, p[u][v]);
             }
-            l = __builtin_fmaf(sum, vsc[ONE ? 0 : u].inv, l);
+            l = __builtin_fmaf(sum * kSumUnit, vsc[ONE ? 0 : u].inv, l);
         };
         auto outputs = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
@@ -701,11 +721,12 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
             top = __builtin_fmaxf(m, top);
             const bool move = top > m + slack;
             if (__any(move)) {
-                const float to = move ? top : m, alpha = __builtin_amdgcn_exp2f(m - (to == kNone ? 0.f : to));
+                const float to = move ? top : m;
+                const Shift shift = shift_of(m - (to == kNone ? 0.f : to));
                 m = to;
-                l *= alpha;
+                l = shift.sum(l);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) o[t] *= alpha;
+                for (int t = 0; t < DT; ++t) o[t] *= shift.all();
             }
         };
         if (plain) {
@@ -769,7 +790,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
         if (h2 == 0) { a.part_ml[2 * slot] = m - lift; a.part_ml[2 * slot + 1] = l; }
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : kSumUnit / l;
     T *dst = (T *)a.out + (s.first + i) * a.o_row + h * a.o_head;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -782,22 +803,15 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
 }
 
 // ---- the slices of a row ------------------------------------------------------------------------------------------------
-// Groups of dim / 4 lanes (rounded up to a power of two) add the slices of a packed row and query head, each in one pass with a
-// running maximum.  Up to kFewSlices one group takes all slices of its own row; beyond, the groups of a workgroup share one
-// row, every group every so many-th slice, and meet in LDS, where the sums are added in group order.
+// Groups of dim / 4 lanes (rounded up to a power of two) add the slices of a packed row and query head, eight loads at a time, the first
+// ones before the weights are known.  A slice's weight comes from its maximum and the common one: lane j of a group (of the wave,
+// where there are more than kFewSlices) has those of slice j and j + 64.  Up to kFewSlices one group takes all slices of its own row;
+// beyond, the groups of a workgroup share one row, every group every so many-th slice, and meet in LDS, where the sums are added
+// in group order.  118 slices of 112 rows of 128: 6.6 us one slice after the other, 8.4 with a pass for the maximum first, 6.9 this way.
 constexpr int kFewSlices = 16;
-struct Joined { float m, l; f32x4_t o; };
-__device__ __forceinline__ void join_one(Joined &j, float m, float l, const f32x4_t &o) {
-    const float top = __builtin_fmaxf(j.m, m), base = top == kNone ? 0.f : top;
-    const float wa = __builtin_amdgcn_exp2f(j.m - base), wb = __builtin_amdgcn_exp2f(m - base);
-    j.o = j.o * wa + o * wb;
-    j.l = __builtin_fmaf(j.l, wa, l * wb);
-    j.m = top;
-}
 template <typename T>
 static __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const AttArgs a) {
     __shared__ f32x4_t meet_o[kBlock];
-    __shared__ float meet_m[16], meet_l[16];
     const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64, groups = kBlock / lanes, group = threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
     const bool shared = a.splits > kFewSlices, live = d < a.kv.dim;
     unsigned blk = shared ? blockIdx.x : blockIdx.x * groups + group;
@@ -812,21 +826,49 @@ static __global__ __launch_bounds__(kBlock) void kvattention_join_kernel(const A
     const int each = slice_tiles(a, last - first), used = last > first ? (last - first + each - 1) / each : 1;
     const int64_t at = (s.first + i) * a.q_heads + h, pitch = a.kv.rows * a.q_heads;
     const float *po = a.part_o + at * a.kv.dim + (live ? d : 0), *pm = a.part_ml + 2 * at;
-    Joined j{kNone, 0.f, {0.f, 0.f, 0.f, 0.f}};
-    const int step = shared ? groups : 1;
-#pragma unroll 4
-    for (int k = shared ? group : 0; k < used; k += step)
-        join_one(j, pm[2 * k * pitch], pm[2 * k * pitch + 1], *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim));
+    const int begin = shared ? group : 0, step = shared ? groups : 1, width = shared ? kWave : lanes, j = threadIdx.x % width;
+    constexpr int kAhead = 8;
+    f32x4_t v[kAhead], o = {0.f, 0.f, 0.f, 0.f};
+    auto load = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const int k = k0 + e * step;
+            v[e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (k < used) v[e] = *reinterpret_cast<const f32x4_t *>(po + k * pitch * a.kv.dim);
+        }
+    };
+    load(begin);
+    const bool one = j < used, two = shared && j + kWave < used;
+    const float m0 = one ? pm[2 * j * pitch] : kNone, m1 = two ? pm[2 * (j + kWave) * pitch] : kNone;
+    const float l0 = one ? pm[2 * j * pitch + 1] : 0.f, l1 = two ? pm[2 * (j + kWave) * pitch + 1] : 0.f;
+    float top = __builtin_fmaxf(m0, m1);
+    for (int x = width / 2; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+    const float base = top == kNone ? 0.f : top;
+    const Shift w0 = shift_of(m0 - base), w1 = shift_of(m1 - base);
+    float l = w0.sum(l0) + w1.sum(l1);
+    for (int x = width / 2; x > 0; x >>= 1) l += __shfl_xor(l, x);
+    for (int k0 = 0; k0 < used; k0 += kAhead * step) {  // the same number of times for all lanes that exchange weights
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {  // past the last slice: a finite weight of zeros
+            const int k = k0 + begin + e * step;
+            float w = __shfl(w0.all(), k, width);
+            if (shared) {
+                const float u = __shfl(w1.all(), k, width);
+                w = k < kWave ? w : u;
+            }
+            o += v[e] * w;
+        }
+        if (k0 + kAhead * step < used) load(k0 + kAhead * step + begin);
+    }
     if (shared) {  // the same for the whole workgroup
-        meet_o[threadIdx.x] = j.o;
-        if (d == 0) { meet_m[group] = j.m; meet_l[group] = j.l; }
+        meet_o[threadIdx.x] = o;
         __syncthreads();
         if (group > 0) return;
-        for (int k = 1; k < groups; ++k) join_one(j, meet_m[k], meet_l[k], meet_o[k * lanes + threadIdx.x]);
+        for (int k = 1; k < groups; ++k) o += meet_o[k * lanes + threadIdx.x];
     }
-    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, j.o[0] * inv, j.o[1] * inv, j.o[2] * inv, j.o[3] * inv);
-    if (d == 0 && a.lse) a.lse[at] = lse_of(j.m, j.l);
+    const float inv = l == 0.f ? 0.f : kSumUnit / l;
+    if (live) store4<T>((T *)a.out + (s.first + i) * a.o_row + h * a.o_head + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (d == 0 && a.lse) a.lse[at] = lse_of(top, l);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------

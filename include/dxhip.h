@@ -578,8 +578,9 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * row, NaN, and so does a scale of a visible token's page that is not finite.  dtype f32 f16 bf16 for q and out (which must
  * not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
  * queries enter the products exactly; a probability, together with its value scale, is rounded to f16, held relative to the
- * largest, for f16 and bf16 rows and kept to 22 bits for f32 rows (values whose page's scale is below 2^-85 of the largest scale
- * met may count as zeros).
+ * largest, for f16 and bf16 rows and kept to 22 bits for f32 rows.  A value scale enters as a power of two: |log2 scale| times
+ * 2^-22 of relative error.  Values whose page's scale is below 2^-85 of the largest that the row sees, or below 2^-92, may lose
+ * precision down to zeros; queries times codes summed over a head must stay finite in fp32.
  * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a
  * second launch: device memory of the caller of at least the query's bytes, 256-byte aligned, that no other call in flight
  * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows and q_heads alone; workspace may be NULL when it is 0. */

@@ -151,7 +151,7 @@ def attention(c, rows, q, scale, causal, window):
     return res
 
 
-def attention_bar(name, c, entry):
+def attention_bar(name, c, entry, far=0.0):
     """How far a result may be from the 64-bit value.  With u = 2^-24:
       score: a product of D exact terms in an fp32 accumulator, each passing through at most D/32 chained and 32 inner additions, and three
       products with scales: (D/32 + 40) u of scale sum|q||k|; f32 rows add 2^-24 of it for the split of q.
@@ -161,10 +161,12 @@ def attention_bar(name, c, entry):
       2^7 times as large for f16 and bf16 rows and 2^15 times for f32 rows, so that f16's smallest steps (half of 2^-24) add at most 2^-32, 2^-40 of
       the largest times a code for each token; of the result: half a step.
       underflow: the hardware's 2^x gives 0 below 2^-126, the smallest normal fp32 number; with l >= 1 (the largest term is 1) each of the N
-      terms is off by at most 2^-126 max|v|."""
+      terms is off by at most 2^-126 max|v|.
+      far: the largest |log2| of the value scales, where they are far from 1.  A scale enters as its logarithm (rounded, and one unit off at most: 3 u
+      far in all) and the sum with the score is rounded (u far), in base 2: ln 2 * 4 u far < 4 u far of a probability and of its share of the sum."""
     out, lse, mag, big, n, top, weight = entry
     u = 2.0 ** -24
-    s = ((c.dim / 32 + 42) * big + 4 * big + 4) * u
+    s = ((c.dim / 32 + 42) * big + 4 * big + 4 + 4 * far) * u
     sums = (n / 32 + 64) * u
     part = {"bf16": 2.0 ** -11, "f16": 2.0 ** -11, "f32": 2.0 ** -22}[name]
     bar = (n * (2.0 ** -40 if name == "f32" else 2.0 ** -32) * float(MAX[c.code]) * weight)[:, None] + mag * (part + 2 * s + 2 * sums)[:, None] + np.abs(out) * HALF_STEP[name] * (1 + 2 ** -8) + TINY[name] + n * 2.0 ** -126 * top

@@ -26,7 +26,7 @@ def call(L, cache, rows_desc, name, q, out, lse, scale, causal, window, st=None,
     return ws
 
 
-def check(L, c, rows, name, q_heads, causal=1, window=0, scale=None, q=None, seed=0, size=1.0):
+def check(L, c, rows, name, q_heads, causal=1, window=0, scale=None, q=None, seed=0, size=1.0, far=0.0):
     scale = c.dim ** -0.5 if scale is None else scale
     if q is None:
         q = torch.randn(rows.rows, q_heads, c.dim, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") * size
@@ -40,7 +40,7 @@ def check(L, c, rows, name, q_heads, causal=1, window=0, scale=None, q=None, see
         if r not in want:  # rows behind the last sequence or beyond max_rows
             assert (got[r] == 7.0).all() and (got_lse[r] == 7.0).all(), r
             continue
-        bar, lse_bar = R.attention_bar(name, c, want[r])
+        bar, lse_bar = R.attention_bar(name, c, want[r], far)
         assert np.array_equal(np.isinf(got_lse[r]), np.isinf(want[r][1])), r
         err = np.abs(got[r] - want[r][0])
         worst = float((err / bar).max())
@@ -231,3 +231,87 @@ def test_as_they_are_used_together(dxh, code):
             step = 6 * max(1.0, float(wk.abs().max())) * dim ** 0.5 / 127 / 2 if code == "i8" else 0
             bound = step if code == "i8" else x.abs() * 2 ** -4 + 6 * max(1.0, float(wk.abs().max())) * dim ** 0.5 / 448 * 2 ** -10
             assert ((b - x).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("counts,lengths", [((1,), (1300,)), ((2,), (128,)), ((1, 3), (5000, 200)), ((40,), (1300,)), ((300,), (2600,))], ids=str)
+def test_value_scales_that_are_no_float_apart(dxh, counts, lengths, page, name):
+    """page scales around 2^-91 and 2^55 in one sequence, in either order and in turn, over waves, tiles and slices: the tokens of both weigh the
+    same in the sum of a row, although the ratio of their scales is less than any float; and a row that does not see the large ones has the small
+    ones' values in full"""
+    for order in ("small first", "large first", "in turn"):
+        c = R.Cache("i8", page, 1, 64, len(counts), -(-max(lengths) // page), seed=14)
+        for b, n in enumerate(lengths):
+            for slot in range(c.per_seq):
+                large = {"small first": slot * page >= n // 2, "large first": slot * page < n // 2, "in turn": slot % 2 == 1}[order]
+                c.vs[c.page_of(b, slot)] *= np.float32(2.0 ** 60 if large else 2.0 ** -86)
+        check(dxh, c, R.Rows(counts, lengths), name, 3, far=92)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("vs", [0.0, 2.0 ** -100, 2.0 ** 121])
+def test_sums_at_the_ends_of_the_range(dxh, vs, rows, page):
+    """a row's sum holds 1 / scale of every token: many tokens of the smallest scale that a cache can have, one of the largest"""
+    for length in (1, 20000) if rows == 1 else (40, 9000):
+        c = R.Cache("i8", page, 1, 64, 1, -(-length // page), seed=15)
+        c.vs[:] = vs
+        if vs <= 2.0 ** -100:
+            c.v[:] = 0  # what has that scale: a page of zeros
+        else:
+            c.v[:] = np.clip(c.v, -32, 32)
+        check(dxh, c, R.Rows((rows,), (length,)), "bf16", 1, far=121)
+        check(dxh, c, R.Rows((rows,), (length,)), "f32", 1, size=0.0, far=121)
+
+
+@pytest.mark.parametrize("name,code,page,dim", [("bf16", "i8", 64, 64), ("f16", "e4m3", 128, 128), ("f32", "i8", 16, 256), ("bf16", "e4m3", 32, 80), ("f32", "e4m3", 64, 128), ("bf16", "i8", 64, 256)])
+def test_one_long_sequence_in_many_slices(dxh, name, code, page, dim):
+    c = R.Cache(code, page, 1, dim, 1, -(-40000 // page), seed=16)
+    rows = R.Rows((2,), (39990,))
+    need = C.c_size_t(0)
+    dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], 3, C.byref(need)))
+    assert need.value > 16 * 2 * 3 * (dim + 2) * 4  # more than 16 slices
+    a = check(dxh, c, rows, name, 3)
+    assert torch.equal(a, check(dxh, c, rows, name, 3))
+    check(dxh, c, rows, name, 3, window=30000)
+
+
+@pytest.mark.parametrize("name,code,page,dim,counts,lengths", [("bf16", "i8", 16, 64, (400, 130), (700, 1500)), ("f16", "e4m3", 64, 128, (130, 300), (2000, 300)), ("f32", "e4m3", 16, 64, (200,), (1000,)),
+                                                             ("bf16", "e4m3", 64, 256, (130,), (2200,)), ("f32", "i8", 32, 96, (150, 3), (300, 900)), ("bf16", "i8", 128, 192, (33,), (3000,))], ids=str)
+def test_prompts_in_slices(dxh, name, code, page, dim, counts, lengths):
+    c = R.Cache(code, page, 1, dim, len(counts), -(-max(lengths) // page), seed=17)
+    rows = R.Rows(counts, lengths, extra=1)
+    need = C.c_size_t(0)
+    dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], 2, C.byref(need)))
+    assert need.value > 0
+    a = check(dxh, c, rows, name, 2)
+    assert torch.equal(a, check(dxh, c, rows, name, 2))
+    check(dxh, c, rows, name, 2, window=500)
+    check(dxh, c, rows, name, 2, causal=0)
+
+
+class LargeCache(R.Cache):
+    """The same cache with its pages behind `gap` others in memory, past the reach of 32-bit offsets; what lies in those is whatever was there."""
+
+    def upload(self):
+        gap = (9 << 29) // (self.heads * self.page * self.dim)  # 4.5 GiB of keys
+        self.dev = [torch.empty((gap + t.shape[0], *t.shape[1:]), dtype=torch.from_numpy(t).dtype, device="cuda") for t in (self.k, self.v, self.ks, self.vs)]
+        for d, t in zip(self.dev, (self.k, self.v, self.ks, self.vs)):
+            d[gap:] = torch.from_numpy(t).cuda()
+        self.dev_table = torch.from_numpy(np.where((self.table >= 0) & (self.table < self.pages), self.table + gap, -1).astype(np.int32)).cuda()
+        return dx.KvCache(*[t.data_ptr() for t in self.dev], self.dev_table.data_ptr(), gap + self.pages, self.per_seq, self.page, self.heads, self.dim, R.CODE[self.code])
+
+
+@pytest.mark.parametrize("name,code,page,dim", [("bf16", "i8", 64, 128), ("f16", "e4m3", 128, 64), ("f32", "e4m3", 64, 64), ("bf16", "e4m3", 64, 256), ("bf16", "i8", 16, 64), ("f32", "i8", 128, 80)])
+def test_a_cache_past_32_bit_offsets(dxh, name, code, page, dim):
+    for counts, lengths in (((1, 1, 2, 1), (5000, 64, 700, 0)), ((50, 3), (90, 400))):
+        c = LargeCache(code, page, 2, dim, len(counts), -(-max(lengths) // page), seed=18, missing=[(0, 0, -1)])
+        check(dxh, c, R.Rows(counts, lengths), name, 4)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_many_short_sequences(dxh, page):
+    """more workgroups than the card has places for"""
+    lengths = [1 + 7 * i % 200 for i in range(300)]
+    check(dxh, R.Cache("i8", page, 2, 64, 300, -(-200 // page), seed=19), R.Rows((1,) * 300, lengths), "bf16", 4)

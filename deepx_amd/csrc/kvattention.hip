@@ -46,10 +46,9 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
     a.min_tiles = a.tile_rows == 16 || a.kv.dim > 128 ? 16 : 4;
     a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16, a.min_tiles);
-    if ((int64_t)a.kv.batch * a.kv.heads * a.row_tiles * a.splits > INT32_MAX || (int64_t)a.kv.batch * a.kv.max_rows * q_heads > INT32_MAX) return DXH_ERR_TOO_LARGE;
-    return DXH_OK;
+    const int64_t blocks = (int64_t)a.kv.batch * a.kv.heads * a.row_tiles, joins = a.splits > 1 ? (int64_t)a.kv.batch * a.kv.max_rows * q_heads : 0;
+    return launch_fits(blocks * a.splits, kBlock) && launch_fits(joins, kBlock) ? DXH_OK : DXH_ERR_TOO_LARGE;
 }
-
 
 }  // namespace
 
@@ -68,7 +67,7 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     AttArgs a;
     int rc = plan(cache, rows, dtype, q_heads, a);
     if (rc != DXH_OK) return rc;
-    if ((causal != 0 && causal != 1) || window < 0 || !(scale - scale == 0.f)) return DXH_ERR_ARG;
+    if ((causal != 0 && causal != 1) || window < 0 || !__builtin_isfinite(scale * kLog2e)) return DXH_ERR_ARG;
     const bool used = !kv_nothing(a.kv);
     const int es = dtype_size(dtype);
     if ((rc = kv_heads_check(q, es, used)) != DXH_OK || (rc = kv_heads_check(out, es, used)) != DXH_OK) return rc;

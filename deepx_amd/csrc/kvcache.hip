@@ -280,9 +280,9 @@ __global__ __launch_bounds__(THREADS) void kvcache_read_kernel(const RowsArgs a)
 
 template <typename T, typename Code> int launch(const RowsArgs &a, bool write, hipStream_t st) {
     const int64_t blocks = (int64_t)2 * a.kv.heads * a.slots * a.kv.batch;
-    if (blocks > INT32_MAX) return DXH_ERR_TOO_LARGE;
     // a lane for every 16 codes of a page, as one new row can change the scale of all: one wave or four
     const bool wide = a.kv.page_size * a.kv.dim > 16 * kWave;
+    if (!launch_fits(blocks, wide ? 256 : 64)) return DXH_ERR_TOO_LARGE;
     if (write) {
         if (wide) kvcache_write_kernel<T, Code, 256><<<(unsigned)blocks, 256, 0, st>>>(a);
         else kvcache_write_kernel<T, Code, 64><<<(unsigned)blocks, 64, 0, st>>>(a);

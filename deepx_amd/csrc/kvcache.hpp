@@ -102,9 +102,11 @@ inline int kv_check(const dxh_kvcache *c, const dxh_kvrows *r, int dtype, KvArgs
     if (a.num_pages == 0) a.pages_per_seq = 0;  // no token has a place
     if (r->batch == 0 || r->rows == 0 || r->max_rows == 0) return DXH_OK;
     if (!r->lengths) return DXH_ERR_ARG;
-    if (c->num_pages > 0 && c->pages_per_seq > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return DXH_ERR_ARG;
+    if (c->num_pages > 0 && c->pages_per_seq > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale || c->k == c->v || c->k_scale == c->v_scale)) return DXH_ERR_ARG;
     return DXH_OK;
 }
+// a launch has fewer than 2^32 work items
+inline bool launch_fits(int64_t blocks, int threads) { return blocks * threads <= (int64_t)UINT32_MAX; }
 inline bool kv_nothing(const KvArgs &a) { return a.batch == 0 || a.rows == 0 || a.max_rows == 0; }
 inline int kv_heads_check(const dxh_heads *h, int es, bool used) {
     if (!h || (used && !h->data)) return DXH_ERR_ARG;

@@ -338,7 +338,12 @@ int check(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, i
         while (g < most && g * (rows < 4 * kCUs ? 1 : 4) < s.heads) g *= 2;
         p.groups = g;
     }
-    // a result may lie where its own inputs do, and nowhere else among what the launch touches
+    // a result may lie where its own inputs do, element on element, and nowhere else among what the launch touches
+    auto shifted = [&](const Part &p, const void *in, int64_t row, int64_t head) { return p.out == in && ((rows > 1 && p.o_row != row) || (p.heads > 1 && p.o_head != head)); };
+    for (int i = 0; i < nparts; ++i) {
+        const Part &p = a.part[i];
+        if (rows > 0 && p.heads && (shifted(p, p.x, p.x_row, p.x_head) || (back && shifted(p, p.y_in, p.y_row, p.y_head)))) return DXH_ERR_ARG;
+    }
     for (int i = 0; i < nparts; ++i)
         for (int j = 0; j < nparts; ++j) {
             const Part &p = a.part[i], &q = a.part[j];
@@ -408,7 +413,7 @@ int dxh_normrope(int dtype, const dxh_normrope_part *parts, int nparts, int64_t 
     if (rc != DXH_OK || rows == 0) return rc;
     const int lg = lanes_of(dtype, dim);
     const int64_t s = slots_of(a, nparts, lg), groups = (rows + s - 1) / s;
-    return launch_dtype(dtype, a, nparts, rot, false, lg, (unsigned)std::min<int64_t>(groups, (int64_t)1 << 30), as_stream(stream));
+    return launch_dtype(dtype, a, nparts, rot, false, lg, (unsigned)std::min<int64_t>(groups, (int64_t)1 << 22), as_stream(stream));
 }
 
 int dxh_normrope_backward_workspace_bytes(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, int32_t dim, size_t *bytes) {

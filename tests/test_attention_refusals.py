@@ -139,3 +139,30 @@ def test_kvcache_attention():
     one = kvrows(rows=1, batch=1, max_rows=1)
     assert query(long, one) == OK and n.value > 0
     assert att(long, one) == WORKSPACE and att(long, one, ws=4096, nbytes=n.value - 1) == WORKSPACE and att(long, one, ws=4096 + 16, nbytes=n.value) == WORKSPACE
+
+
+def test_results_laid_out_unlike_the_input_they_replace():
+    """in place only element on element: the same pointer with other strides is refused where a stride is used at all"""
+    L = dx.load()
+    same = lambda rows, n, row=1024, head=64, **kw: L.dxh_normrope(dx.BF16, (dx.NormropePart * 1)(norm_part(x=heads(4096), y=heads(4096, row, head), heads=n, **kw)), 1, rows, 64, 1e-6, rotary(cos=None), None)  # noqa: E731
+    assert same(2, 4, row=2048) == ARG and same(1, 4, head=128) == ARG
+    back = lambda dx_: L.dxh_normrope_backward(dx.BF16, (dx.NormropePart * 1)(norm_part(x=heads(4096), y=heads(8192), dx=dx_)), 1, 2, 64, 1e-6, None, 4096, 1 << 30, None)  # noqa: E731
+    assert back(heads(8192, row=2048)) == ARG and back(heads(4096, head=128)) == ARG
+
+
+def test_caches_whose_halves_are_one():
+    L = dx.load()
+    for kw in (dict(v=4096), dict(v_scale=256)):
+        for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
+            assert fn(cache(**kw), kvrows(rows=1), dx.BF16, heads(), heads(16384), None) == ARG, kw
+        assert L.dxh_kvcache_attention(cache(**kw), kvrows(rows=1), dx.BF16, 14, heads(), heads(8192), None, 0.125, 1, 0, None, 0, None) == ARG, kw
+
+
+def test_sizes_past_one_launch():
+    """a launch has fewer than 2^32 work items; a score scale is finite in base 2 too"""
+    L, big = dx.load(), -6
+    n = C.c_size_t(1)
+    rows = kvrows(rows=1 << 26, batch=1 << 23, max_rows=8)
+    assert L.dxh_kvcache_write(cache(), rows, dx.BF16, heads(), heads(16384), None) == big  # 2^23 sequences, 2 heads, keys and values, 2 pages each, 64 lanes
+    assert L.dxh_kvcache_attention_workspace_bytes(cache(), kvrows(rows=1 << 24, batch=1 << 23, max_rows=1), dx.BF16, 14, C.byref(n)) == big
+    assert L.dxh_kvcache_attention(cache(), kvrows(rows=1), dx.BF16, 14, heads(), heads(8192), None, 3e38, 1, 0, None, 0, None) == ARG

@@ -17,7 +17,7 @@ constexpr int64_t kFewRows = 32;  // rows of one sequence and key head up to whi
 //   256, 57 us uncut and 67 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
 //   7 / 1 heads of 64: 82 us uncut, 39 in slices).
 int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few, int min_tiles) {
-    const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles, tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
+    const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles * (few ? 1 : value_parts(kv.dim)), tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
     int64_t want;
     if (few) want = ((kv.batch > 1 ? 8 : 2) * kCUs + blocks - 1) / blocks;
     else want = blocks < 2 * kCUs ? (4 * kCUs + blocks - 1) / blocks : 1;
@@ -46,7 +46,7 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
     a.min_tiles = a.tile_rows == 16 || a.kv.dim > 128 ? 16 : 4;
     a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16, a.min_tiles);
-    const int64_t blocks = (int64_t)a.kv.batch * a.kv.heads * a.row_tiles, joins = a.splits > 1 ? (int64_t)a.kv.batch * a.kv.max_rows * q_heads : 0;
+    const int64_t blocks = (int64_t)a.kv.batch * a.kv.heads * a.row_tiles * (a.tile_rows == 16 ? 1 : value_parts(a.kv.dim)), joins = a.splits > 1 ? (int64_t)a.kv.batch * a.kv.max_rows * q_heads : 0;
     return launch_fits(blocks * a.splits, kBlock) && launch_fits(joins, kBlock) ? DXH_OK : DXH_ERR_TOO_LARGE;
 }
 

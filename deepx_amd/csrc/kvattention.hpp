@@ -473,18 +473,24 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
 // TFLOP/s), matrix pipe busy 31 %, vector pipe 45 % (2^x a third of that), waves waiting 34 %.  Eight waves a workgroup, two
 // buffers with one barrier a tile, an enforced alternation of matrix and vector instructions, and raised wave priority under
 // the products were measured at 682, 672, 669 and 674 us.
+// Heads over 128: two workgroups take half of the output's dimensions each and both compute the scores: half as much again in
+// products, but a row's registers are fewer.  Four prompts of 2k-3k tokens, 16 / 4 heads of 256: 959 us with the head in one
+// workgroup, 805 in two with one wave a SIMD, 535 with two.  Where every lane has page numbers of its own (pages of 16 and 32) the
+// second wave costs more in spilled registers than it hides: eight prompts of 313-364 tokens 47 us, 44 with one.
+constexpr int value_parts(int padded_dim) { return padded_dim > 128 ? 2 : 1; }
 template <typename T, typename Code, int DP, bool EXACT, bool ONE, int WAVES>
-static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && RowType<T>::QP == 1) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
+static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP == 1 && (ONE || DP == 128)) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
-    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = DP / 32, THREADS = WAVES * kWave;
-    constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, PIECES = (DP * 4 + THREADS - 1) / THREADS;
+    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, PARTS = value_parts(DP), DV = DP / PARTS, DT = DV / 32, THREADS = WAVES * kWave;
+    constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, KPIECES = (DP * 4 + THREADS - 1) / THREADS, VPIECES = (DV * 4 + THREADS - 1) / THREADS;
     constexpr float slack = PP == 1 ? kSlack : 0.f, lift = kLift - slack;
-    __shared__ __attribute__((aligned(16))) unsigned char kl[64 * KPITCH], vl[DP * VPITCH];
+    __shared__ __attribute__((aligned(16))) unsigned char kl[64 * KPITCH], vl[DV * VPITCH];
     __shared__ uint32_t bad_tokens[2][2];
     // longest tiles of rows first; the tiles of one (sequence, head) stay on one XCD when there are a multiple of 8 pairs
     const unsigned pairs = (unsigned)a.kv.batch * a.kv.heads;
     unsigned blk = blockIdx.x;
     const int pair = blk % pairs; blk /= pairs;
+    const int part = blk % PARTS; blk /= PARTS;
     const int split = blk % (unsigned)a.splits, rt = a.row_tiles - 1 - (int)(blk / (unsigned)a.splits);
     const int head = pair % a.kv.heads, seq = pair / a.kv.heads;
     const KvSeq s = kv_seq(a.kv, seq);
@@ -496,29 +502,36 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
     tile_range(a, s, r0 / G, (r0 + WAVES * 32 - 1) / G, tile, tile_end);
     if (!slice_of(a, split, tile, tile_end)) return;
 
-    // pieces of 16 codes that this thread brings: of the keys token kt, dimensions kd ..; of the values dimension vd, tokens vt ..
-    int kt[PIECES], kd[PIECES], vd[PIECES], vt[PIECES];
-    uint32_t kofs[PIECES], vofs[PIECES];  // where the pieces lie in a page of this head, for tiles that begin in a page's first 64 tokens
-    bool there[PIECES];
+    // pieces of 16 codes that this thread brings: of the keys token kt, dimensions kd ..; of the values dimension v0 + vd, tokens vt ..
+    const int v0 = part * DV, Dv = EXACT || D - v0 > DV ? DV : D - v0;
+    int kt[KPIECES], kd[KPIECES], vd[VPIECES], vt[VPIECES];
+    uint32_t kofs[KPIECES], vofs[VPIECES];  // where the pieces lie in a page of this head, for tiles that begin in a page's first 64 tokens
+    bool kthere[KPIECES], vthere[VPIECES];  // others load piece 0 and drop it
 #pragma unroll
-    for (int j = 0; j < PIECES; ++j) {
+    for (int j = 0; j < KPIECES; ++j) {
         const int id = threadIdx.x + j * THREADS, per = D / 16;
-        there[j] = EXACT || id < 4 * D;  // others load piece 0 and drop it
-        const int x = there[j] ? id : 0;
+        kthere[j] = EXACT || id < 4 * D;
+        const int x = kthere[j] ? id : 0;
         kt[j] = x / per;
         kd[j] = (x - kt[j] * per) * 16;
-        // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
-        vd[j] = P == 16 ? x % D : x >> 2;
-        vt[j] = (P == 16 ? x / D : x & 3) * 16;
         kofs[j] = (kt[j] & (P - 1)) * D + kd[j];
-        vofs[j] = vd[j] * P + (vt[j] & (P - 1));
+    }
+#pragma unroll
+    for (int j = 0; j < VPIECES; ++j) {
+        const int id = threadIdx.x + j * THREADS;
+        vthere[j] = EXACT || id < 4 * Dv;
+        const int x = vthere[j] ? id : 0;
+        // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
+        vd[j] = P == 16 ? x % Dv : x >> 2;
+        vt[j] = (P == 16 ? x / Dv : x & 3) * 16;
+        vofs[j] = (v0 + vd[j]) * P + (vt[j] & (P - 1));
     }
     if (threadIdx.x < 4) bad_tokens[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     if (D < DP) {  // what pads the head stays zero
         for (int id = threadIdx.x; id < 64 * (DP - D) / 8; id += THREADS)
             *reinterpret_cast<u32x4 *>(kl + (id / ((DP - D) / 8)) * KPITCH + D * 2 + (id % ((DP - D) / 8)) * 16) = u32x4{0u, 0u, 0u, 0u};
-        for (int id = threadIdx.x; id < (DP - D) * 8; id += THREADS)
-            *reinterpret_cast<u32x4 *>(vl + (D + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
+        for (int id = threadIdx.x; id < (DV - Dv) * 8; id += THREADS)
+            *reinterpret_cast<u32x4 *>(vl + (Dv + id / 8) * VPITCH + (id % 8) * 16) = u32x4{0u, 0u, 0u, 0u};
     }
 
     // this lane's row
@@ -553,20 +566,19 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
 
     // table entries two tiles ahead, codes and scales one.  ONE: a tile lies in one page, whose number, address and scales are the
     // same for all lanes and stay in scalar registers.
-    constexpr int E = ONE ? 1 : PIECES, S = ONE ? 1 : 2;
-    int kentry[E], ventry[E], sentry[S], sp[S];
-    bool vnone[E];  // values: the page is none
-    u32x4 kc[PIECES], vc[PIECES];
+    constexpr int KE = ONE ? 1 : KPIECES, VE = ONE ? 1 : VPIECES, S = ONE ? 1 : 2;
+    int kentry[KE], ventry[VE], sentry[S], sp[S];
+    bool vnone[VE];  // values: the page is none
+    u32x4 kc[KPIECES], vc[VPIECES];
     float ks_next[S], vs_next[S];
     auto entries = [&](int t) __attribute__((always_inline)) {
         if constexpr (ONE) {
             kentry[0] = entry_at(a, seq, t * 64);
         } else {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                kentry[j] = entry_at(a, seq, t * 64 + kt[j]);
-                ventry[j] = entry_at(a, seq, t * 64 + vt[j]);
-            }
+            for (int j = 0; j < KPIECES; ++j) kentry[j] = entry_at(a, seq, t * 64 + kt[j]);
+#pragma unroll
+            for (int j = 0; j < VPIECES; ++j) ventry[j] = entry_at(a, seq, t * 64 + vt[j]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) sentry[u] = entry_at(a, seq, t * 64 + u * 32 + h2 * 16);
         }
@@ -581,16 +593,19 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
             const int page = sp[0] < 0 ? 0 : sp[0];
             const uint8_t *ksrc = khead + page * page_bytes + half * D, *vsrc = vhead + page * page_bytes + half;
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                kc[j] = *reinterpret_cast<const u32x4 *>(ksrc + kofs[j]);
-                vc[j] = *reinterpret_cast<const u32x4 *>(vsrc + vofs[j]);
-            }
+            for (int j = 0; j < KPIECES; ++j) kc[j] = *reinterpret_cast<const u32x4 *>(ksrc + kofs[j]);
+#pragma unroll
+            for (int j = 0; j < VPIECES; ++j) vc[j] = *reinterpret_cast<const u32x4 *>(vsrc + vofs[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                const int kp = page_of(a, s, kentry[j], t * 64 + kt[j]), vp = page_of(a, s, ventry[j], t * 64 + vt[j]);
-                vnone[j] = vp < 0;
+            for (int j = 0; j < KPIECES; ++j) {
+                const int kp = page_of(a, s, kentry[j], t * 64 + kt[j]);
                 kc[j] = *reinterpret_cast<const u32x4 *>(khead + (kp < 0 ? 0 : kp) * page_bytes + (kofs[j] + half * D));
+            }
+#pragma unroll
+            for (int j = 0; j < VPIECES; ++j) {
+                const int vp = page_of(a, s, ventry[j], t * 64 + vt[j]);
+                vnone[j] = vp < 0;
                 vc[j] = *reinterpret_cast<const u32x4 *>(vhead + (vp < 0 ? 0 : vp) * page_bytes + (vofs[j] + half));
             }
 #pragma unroll
@@ -608,12 +623,12 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
         if constexpr (std::is_same_v<Code, CodeE4M3>) {
             bool gone = false;
 #pragma unroll
-            for (int j = 0; j < E; ++j) gone = gone || vnone[j];
+            for (int j = 0; j < VE; ++j) gone = gone || vnone[j];
             const bool cut = t * 64 < group_all.lo || t * 64 + 64 > group_all.hi;
             if (cut || __any(gone)) {
 #pragma unroll
-                for (int j = 0; j < PIECES; ++j) {
-                    if (!there[j]) continue;
+                for (int j = 0; j < VPIECES; ++j) {
+                    if (!vthere[j]) continue;
                     if (vnone[ONE ? 0 : j]) vc[j] = u32x4{0u, 0u, 0u, 0u};
                     const uint32_t found = cut ? drop_nans(vc[j]) : 0u;
                     if (found) atomicOr(&bad_tokens[t & 1][vt[j] >> 5], found << (vt[j] & 16));
@@ -624,12 +639,16 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
     // the codes in the registers as operands into LDS
     auto stage = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            if (!there[j]) continue;
+        for (int j = 0; j < KPIECES; ++j) {
+            if (!kthere[j]) continue;
             u32x4 *dst = reinterpret_cast<u32x4 *>(kl + kt[j] * KPITCH + kd[j] * 2);
             dst[0] = codes8<Code, Kind>(kc[j][0], kc[j][1]);
             dst[1] = codes8<Code, Kind>(kc[j][2], kc[j][3]);
-            dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
+        }
+#pragma unroll
+        for (int j = 0; j < VPIECES; ++j) {
+            if (!vthere[j]) continue;
+            u32x4 *dst = reinterpret_cast<u32x4 *>(vl + vd[j] * VPITCH + vt[j] * 2);
             dst[0] = codes8<Code, _Float16>(vc[j][0], vc[j][1]);
             dst[1] = codes8<Code, _Float16>(vc[j][2], vc[j][3]);
         }
@@ -784,10 +803,10 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const int d = t * 32 + b * 8 + h2 * 4;
+                const int d = v0 + t * 32 + b * 8 + h2 * 4;
                 if (d < D) *reinterpret_cast<f32x4_t *>(a.part_o + slot * D + d) = f32x4_t{o[t][4 * b], o[t][4 * b + 1], o[t][4 * b + 2], o[t][4 * b + 3]};
             }
-        if (h2 == 0) { a.part_ml[2 * slot] = m - lift; a.part_ml[2 * slot + 1] = l; }
+        if (h2 == 0 && part == 0) { a.part_ml[2 * slot] = m - lift; a.part_ml[2 * slot + 1] = l; }
         return;
     }
     const float inv = l == 0.f ? 0.f : kSumUnit / l;
@@ -796,10 +815,10 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (DP == 128 && Row
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int d = t * 32 + b * 8 + h2 * 4;
+            const int d = v0 + t * 32 + b * 8 + h2 * 4;
             if (d < D) store4<T>(dst + d, o[t][4 * b] * inv, o[t][4 * b + 1] * inv, o[t][4 * b + 2] * inv, o[t][4 * b + 3] * inv);
         }
-    if (h2 == 0 && a.lse) a.lse[at] = lse_of(m - lift, l);
+    if (h2 == 0 && part == 0 && a.lse) a.lse[at] = lse_of(m - lift, l);
 }
 
 // ---- the slices of a row ------------------------------------------------------------------------------------------------
@@ -884,14 +903,17 @@ template <typename T, typename Code, int SPANS, bool EXACT, bool ONE> void launc
         }
         kvattention_rows_kernel<T, Code, SPANS, EXACT, ONE, false, 4><<<blocks, kBlock, 0, st>>>(a);
     } else {
-        kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks, kWaves * kWave, 0, st>>>(a);
+        kvattention_tiles_kernel<T, Code, SPANS * 64, EXACT, ONE, kWaves><<<blocks * value_parts(SPANS * 64), kWaves * kWave, 0, st>>>(a);
     }
 }
-// head sizes that fill their registers need no bounds in the loops, pages of at least 64 tokens no page number a lane
+// Head sizes that fill their registers need no bounds in the loops, pages of at least 64 tokens no page number a lane.  Four prompts of
+// 2k-3k tokens, 16 / 4 heads of 96, pages of 64: 174 us, with a page number a lane 261.
 template <typename T, typename Code, int SPANS> void launch_dim(const AttArgs &a, hipStream_t st) {
-    if (a.kv.dim != SPANS * 64) launch_one<T, Code, SPANS, false, false>(a, st);
-    else if (a.kv.page_size < 64) launch_one<T, Code, SPANS, true, false>(a, st);
-    else launch_one<T, Code, SPANS, true, true>(a, st);
+    const bool exact = a.kv.dim == SPANS * 64, one = a.kv.page_size >= 64;
+    if (exact && one) launch_one<T, Code, SPANS, true, true>(a, st);
+    else if (exact) launch_one<T, Code, SPANS, true, false>(a, st);
+    else if (one) launch_one<T, Code, SPANS, false, true>(a, st);
+    else launch_one<T, Code, SPANS, false, false>(a, st);
 }
 template <typename T, typename Code> int kvattention_launch(const AttArgs &a, hipStream_t st) {
     if (a.kv.dim <= 64) launch_dim<T, Code, 1>(a, st);

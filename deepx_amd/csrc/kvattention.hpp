@@ -507,6 +507,10 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP =
     int kt[KPIECES], kd[KPIECES], vd[VPIECES], vt[VPIECES];
     uint32_t kofs[KPIECES], vofs[VPIECES];  // where the pieces lie in a page of this head, for tiles that begin in a page's first 64 tokens
     bool kthere[KPIECES], vthere[VPIECES];  // others load piece 0 and drop it
+    // a token of the piece's page: the same for a whole wave, whose pieces are 4, 8 or 16 tokens' keys and one block of tokens' values,
+    // where the head fills its registers, so that page numbers and addresses are scalar
+    int kpage[KPIECES], vpage[VPIECES];
+    auto of_wave = [](int token) __attribute__((always_inline)) { return EXACT ? __builtin_amdgcn_readfirstlane(token) : token; };
 #pragma unroll
     for (int j = 0; j < KPIECES; ++j) {
         const int id = threadIdx.x + j * THREADS, per = D / 16;
@@ -514,6 +518,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP =
         const int x = kthere[j] ? id : 0;
         kt[j] = x / per;
         kd[j] = (x - kt[j] * per) * 16;
+        kpage[j] = of_wave(kt[j]);
         kofs[j] = (kt[j] & (P - 1)) * D + kd[j];
     }
 #pragma unroll
@@ -521,9 +526,10 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP =
         const int id = threadIdx.x + j * THREADS;
         vthere[j] = EXACT || id < 4 * Dv;
         const int x = vthere[j] ? id : 0;
-        // lanes along the dimensions in small pages ([dim][16]: one run of bytes), along the tokens in larger ones
-        vd[j] = P == 16 ? x % Dv : x >> 2;
-        vt[j] = (P == 16 ? x / Dv : x & 3) * 16;
+        // lanes along the tokens where a page holds them all, else along the dimensions: one page a wave
+        vd[j] = ONE ? x >> 2 : x % Dv;
+        vt[j] = (ONE ? x & 3 : x / Dv) * 16;
+        vpage[j] = of_wave(vt[j]);
         vofs[j] = (v0 + vd[j]) * P + (vt[j] & (P - 1));
     }
     if (threadIdx.x < 4) bad_tokens[threadIdx.x >> 1][threadIdx.x & 1] = 0;
@@ -576,9 +582,9 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP =
             kentry[0] = entry_at(a, seq, t * 64);
         } else {
 #pragma unroll
-            for (int j = 0; j < KPIECES; ++j) kentry[j] = entry_at(a, seq, t * 64 + kt[j]);
+            for (int j = 0; j < KPIECES; ++j) kentry[j] = entry_at(a, seq, t * 64 + kpage[j]);
 #pragma unroll
-            for (int j = 0; j < VPIECES; ++j) ventry[j] = entry_at(a, seq, t * 64 + vt[j]);
+            for (int j = 0; j < VPIECES; ++j) ventry[j] = entry_at(a, seq, t * 64 + vpage[j]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) sentry[u] = entry_at(a, seq, t * 64 + u * 32 + h2 * 16);
         }
@@ -599,12 +605,12 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP =
         } else {
 #pragma unroll
             for (int j = 0; j < KPIECES; ++j) {
-                const int kp = page_of(a, s, kentry[j], t * 64 + kt[j]);
+                const int kp = page_of(a, s, kentry[j], t * 64 + kpage[j]);
                 kc[j] = *reinterpret_cast<const u32x4 *>(khead + (kp < 0 ? 0 : kp) * page_bytes + (kofs[j] + half * D));
             }
 #pragma unroll
             for (int j = 0; j < VPIECES; ++j) {
-                const int vp = page_of(a, s, ventry[j], t * 64 + vt[j]);
+                const int vp = page_of(a, s, ventry[j], t * 64 + vpage[j]);
                 vnone[j] = vp < 0;
                 vc[j] = *reinterpret_cast<const u32x4 *>(vhead + (vp < 0 ? 0 : vp) * page_bytes + (vofs[j] + half));
             }

@@ -475,11 +475,10 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
 // the products were measured at 682, 672, 669 and 674 us.
 // Heads over 128: two workgroups take half of the output's dimensions each and both compute the scores: half as much again in
 // products, but a row's registers are fewer.  Four prompts of 2k-3k tokens, 16 / 4 heads of 256: 959 us with the head in one
-// workgroup, 805 in two with one wave a SIMD, 535 with two.  Where every lane has page numbers of its own (pages of 16 and 32) the
-// second wave costs more in spilled registers than it hides: eight prompts of 313-364 tokens 47 us, 44 with one.
+// workgroup, 805 in two with one wave a SIMD, 535 with two (960, 740 where pages are of 16 tokens).
 constexpr int value_parts(int padded_dim) { return padded_dim > 128 ? 2 : 1; }
 template <typename T, typename Code, int DP, bool EXACT, bool ONE, int WAVES>
-static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || (RowType<T>::QP == 1 && (ONE || DP == 128)) ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
+static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || RowType<T>::QP == 1 ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
     constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, PARTS = value_parts(DP), DV = DP / PARTS, DT = DV / 32, THREADS = WAVES * kWave;
     constexpr int KPITCH = DP * 2 + 16, VPITCH = 64 * 2 + 16, KPIECES = (DP * 4 + THREADS - 1) / THREADS, VPIECES = (DV * 4 + THREADS - 1) / THREADS;

@@ -315,3 +315,39 @@ def test_many_short_sequences(dxh, page):
     """more workgroups than the card has places for"""
     lengths = [1 + 7 * i % 200 for i in range(300)]
     check(dxh, R.Cache("i8", page, 2, 64, 300, -(-200 // page), seed=19), R.Rows((1,) * 300, lengths), "bf16", 4)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("page,dim", [(64, 64), (64, 128), (64, 256), (16, 256), (64, 80), (128, 192), (32, 128), (128, 96)])
+def test_unseen_tokens_have_no_effect_at_other_sizes(dxh, page, dim, name):
+    """the worst codes and scales where no row sees them, over prompts, chunks and single rows, for pages that hold a tile and heads that leave
+    registers empty or are shared by two workgroups"""
+    per = -(-260 // page)
+    for rows in (R.Rows((50, 70, 3, 0), (230, 70, 1, 5), extra=1), R.Rows((1, 2, 1, 1), (200, 260, 0, 2 ** 31 - 1))):
+        c = R.Cache("e4m3", page, 1, dim, 4, per, seed=20, missing=[(0, 1, -1), (1, 0, 1 << 30), (3, per - 1, -7)])
+        seen = np.zeros((c.pages, page), bool)
+        for b, r, t in rows.each():
+            for j in range(0, min(t + 1, rows.lengths[b], per * page) if t >= 0 else 0):
+                if c.page_of(b, j // page) >= 0:
+                    seen[c.page_of(b, j // page), j % page] = True
+        c.k[~np.broadcast_to(seen[:, None, :, None], c.k.shape)] = 127
+        c.v[~np.broadcast_to(seen[:, None, None, :], c.v.shape)] = -1
+        c.ks[~seen.any(1)] = np.nan
+        c.vs[~seen.any(1)] = -np.inf
+        check(dxh, c, rows, name, 3)
+
+
+@pytest.mark.parametrize("page,dim", [(64, 64), (64, 256), (16, 256), (128, 192), (64, 80)])
+def test_a_nan_among_values_reaches_only_rows_that_see_it(dxh, page, dim):
+    c = R.Cache("e4m3", page, 1, dim, 1, -(-300 // page), seed=21)
+    rows = R.Rows((120,), (290,))
+    q = torch.randn(120, 2, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    clean = check(dxh, c, rows, "bf16", 2, q=q)
+    for d in (0, dim - 1):
+        keep = c.v.copy()
+        c.v[c.page_of(0, 200 // page), 0, d, 200 % page] = 127
+        out = torch.full_like(clean, 7.0)
+        call(dxh, c.upload(), rows.upload(), "bf16", q.bfloat16(), out, None, dim ** -0.5, 1, 0)
+        sees = torch.arange(120) + 170 >= 200
+        assert torch.equal(out[~sees], clean[~sees]) and torch.isnan(out[sees][..., d]).all()
+        c.v = keep

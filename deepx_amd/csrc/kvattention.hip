@@ -5,7 +5,19 @@ using namespace dxh;
 
 namespace {
 
-constexpr int64_t kFewRows = 32;  // rows of one sequence and key head up to which the 16-row kernel runs
+// Which of the two kernels; `rows` of one sequence and key head.  The 16-row kernel decodes a tile of codes for every 16 rows, the other for
+// every 128, but padded to that many rows and a tile at a time behind two barriers.  16-row against 128-row kernel, bf16 unless said:
+//   up to 32 rows always; up to 96 f32 rows, whose products cost more than the codes (48 rows over 3k-8k tokens, 16 x 4 heads of
+//   128: 64 and 122 us; bf16, 35 rows over 4k-8k, 16 x 8 heads: 101 and 93);
+//   else where the 128-row tiles leave a third of the CUs idle and there is little work, at most 64 products of a 16-row and a 64-token tile a CU: a prompt
+//   of 512 tokens, 16 / 4 heads of 128, 13.0 and 23.4; a prompt of 300, f32, 2 / 1 heads of 80, 9.7 and 25.6; but four f32 prompts of
+//   2000, 8 / 2 heads of 128 (128 products a CU), 132 and 114, and eight prompts of 128, 32 / 8 heads of 128 (as many 128-row tiles as
+//   CUs), 29.8 and 14.7; eight of 313-364, 8 heads of 256, 77 and 43.
+bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
+    if (rows <= (dtype == DXH_F32 ? 96 : 32)) return true;
+    const int64_t tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64, pairs = (int64_t)kv.batch * kv.heads;
+    return 3 * pairs * ((rows + kTileRows - 1) / kTileRows) * value_parts(kv.dim) <= 2 * kCUs && pairs * ((rows + 15) / 16) * tiles <= 64 * kCUs;
+}
 
 // How many slices the tokens of a sequence are cut into, counted on the longest sequence that the cache can hold; a slice has at
 // least min_tiles tiles (slice_tiles), so that short sequences use fewer.
@@ -42,7 +54,7 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     if (kv_nothing(a.kv)) return DXH_OK;
     const int64_t most = (int64_t)a.kv.max_rows * a.group;
     if (most > INT32_MAX - kTileRows) return DXH_ERR_TOO_LARGE;
-    a.tile_rows = most <= kFewRows ? 16 : kTileRows;
+    a.tile_rows = few_rows(a.kv, most, dtype) ? 16 : kTileRows;
     a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
     a.min_tiles = a.tile_rows == 16 || a.kv.dim > 128 ? 16 : 4;
     a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16, a.min_tiles);

@@ -583,7 +583,7 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * precision down to zeros; queries times codes summed over a head must stay finite in fp32.
  * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a
  * second launch: device memory of the caller of at least the query's bytes, 256-byte aligned, that no other call in flight
- * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows and q_heads alone; workspace may be NULL when it is 0. */
+ * uses.  The query's answer depends on cache, rows->batch, rows->rows, rows->max_rows, dtype and q_heads alone; workspace may be NULL when it is 0. */
 DXH_API int dxh_kvcache_attention_workspace_bytes(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_heads, size_t *bytes);
 DXH_API int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_heads, const dxh_heads *q,
                                   const dxh_heads *out, float *lse, float scale, int causal, int64_t window, void *workspace,

@@ -282,9 +282,15 @@ def test_one_long_sequence_in_many_slices(dxh, name, code, page, dim):
 def test_prompts_in_slices(dxh, name, code, page, dim, counts, lengths):
     c = R.Cache(code, page, 1, dim, len(counts), -(-max(lengths) // page), seed=17)
     rows = R.Rows(counts, lengths, extra=1)
+    a = check(dxh, c, rows, name, 2)
+    assert torch.equal(a, check(dxh, c, rows, name, 2))
+    check(dxh, c, rows, name, 2, window=500)
+    check(dxh, c, rows, name, 2, causal=0)
+    # as many tiles of rows as leave some CUs idle, with more work than the kernel for few rows is given: slices of the other one
+    rows.max_rows = 255 * 128 // 2 // len(counts)
     need = C.c_size_t(0)
     dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], 2, C.byref(need)))
-    assert need.value > 0
+    assert need.value > 0 or max(lengths) < 600 or dim > 128
     a = check(dxh, c, rows, name, 2)
     assert torch.equal(a, check(dxh, c, rows, name, 2))
     check(dxh, c, rows, name, 2, window=500)
@@ -308,6 +314,7 @@ def test_a_cache_past_32_bit_offsets(dxh, name, code, page, dim):
     for counts, lengths in (((1, 1, 2, 1), (5000, 64, 700, 0)), ((50, 3), (90, 400))):
         c = LargeCache(code, page, 2, dim, len(counts), -(-max(lengths) // page), seed=18, missing=[(0, 0, -1)])
         check(dxh, c, R.Rows(counts, lengths), name, 4)
+        check(dxh, c, many(counts, lengths), name, 4)
 
 
 @pytest.mark.parametrize("page", [16, 64])
@@ -351,3 +358,77 @@ def test_a_nan_among_values_reaches_only_rows_that_see_it(dxh, page, dim):
         sees = torch.arange(120) + 170 >= 200
         assert torch.equal(out[~sees], clean[~sees]) and torch.isnan(out[sees][..., d]).all()
         c.v = keep
+
+
+# The host chooses the kernel by the rows that a sequence can have; with room for this many it is the one for many rows, whatever there is.
+def many(counts, lengths, extra=0):
+    return R.Rows(counts, lengths, extra=extra, max_rows=1 << 15)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("case", CASES + [("i8", 64, 1, 3, 64, (130, 1), (200, 70)), ("e4m3", 32, 2, 2, 128, (129, 40), (129, 300)), ("i8", 128, 1, 2, 256, (100,), (300,)), ("e4m3", 16, 1, 2, 224, (40, 90), (50, 200)),
+                                          ("i8", 64, 1, 2, 96, (70,), (190,)), ("e4m3", 32, 1, 1, 256, (33,), (100,))], ids=str)
+def test_ragged_many(dxh, case, name):
+    code, page, hk, hq, dim, counts, lengths = case
+    c = R.Cache(code, page, hk, dim, len(counts), -(-max(lengths) // page), seed=dim + hq + 1)
+    check(dxh, c, many(counts, lengths, extra=1), name, hq)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [0, 1])
+@pytest.mark.parametrize("window", [0, 1, 63, 64, 65, 200])
+@pytest.mark.parametrize("code,page", [("i8", 16), ("e4m3", 64)])
+def test_masks_many(dxh, code, page, window, causal, name):
+    c = R.Cache(code, page, 1, 64, 3, -(-320 // page), seed=window % 97 + 1)
+    check(dxh, c, many((70, 1, 33), (300, 257, 33)), name, 3, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 64), (64, 128), (64, 256), (16, 256), (64, 80), (128, 192), (32, 128), (128, 96)])
+def test_unseen_tokens_many(dxh, page, dim, name):
+    per = -(-260 // page)
+    for rows in (many((50, 70, 3, 0), (230, 70, 1, 5), extra=1), many((1, 2, 1, 1), (200, 260, 0, 2 ** 31 - 1))):
+        c = R.Cache("e4m3", page, 1, dim, 4, per, seed=22, missing=[(0, 1, -1), (1, 0, 1 << 30), (3, per - 1, -7)])
+        seen = np.zeros((c.pages, page), bool)
+        for b, r, t in rows.each():
+            for j in range(0, min(t + 1, rows.lengths[b], per * page) if t >= 0 else 0):
+                if c.page_of(b, j // page) >= 0:
+                    seen[c.page_of(b, j // page), j % page] = True
+        c.k[~np.broadcast_to(seen[:, None, :, None], c.k.shape)] = 127
+        c.v[~np.broadcast_to(seen[:, None, None, :], c.v.shape)] = -1
+        c.ks[~seen.any(1)] = np.nan
+        c.vs[~seen.any(1)] = -np.inf
+        check(dxh, c, rows, name, 3)
+
+
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 64), (64, 256), (16, 256), (128, 192), (64, 80)])
+def test_a_nan_among_values_many(dxh, page, dim):
+    c = R.Cache("e4m3", page, 1, dim, 1, -(-300 // page), seed=23)
+    rows = many((120,), (290,))
+    q = torch.randn(120, 2, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    clean = check(dxh, c, rows, "bf16", 2, q=q)
+    for d in (0, dim - 1):
+        keep = c.v.copy()
+        c.v[c.page_of(0, 200 // page), 0, d, 200 % page] = 127
+        out = torch.full_like(clean, 7.0)
+        call(dxh, c.upload(), rows.upload(), "bf16", q.bfloat16(), out, None, dim ** -0.5, 1, 0)
+        sees = torch.arange(120) + 170 >= 200
+        assert torch.equal(out[~sees], clean[~sees]) and torch.isnan(out[sees][..., d]).all()
+        c.v = keep
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [16, 64])
+def test_value_scales_many(dxh, page, name):
+    """scales that are no float apart, and sums at the ends of their range"""
+    for order in ("small first", "large first", "in turn"):
+        c = R.Cache("i8", page, 1, 64, 1, -(-1300 // page), seed=24)
+        for slot in range(c.per_seq):
+            large = {"small first": slot * page >= 650, "large first": slot * page < 650, "in turn": slot % 2 == 1}[order]
+            c.vs[c.page_of(0, slot)] *= np.float32(2.0 ** 60 if large else 2.0 ** -86)
+        check(dxh, c, many((40,), (1300,)), name, 3, far=92)
+    for vs in (0.0, 2.0 ** 121):
+        c = R.Cache("i8", page, 1, 64, 1, -(-9000 // page), seed=25)
+        c.vs[:] = vs
+        c.v[:] = 0 if vs == 0 else np.clip(c.v, -32, 32)
+        check(dxh, c, many((40,), (9000,)), name, 1, size=0.0, far=121)

@@ -26,7 +26,7 @@ bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
 //   two workgroups a CU (131071 tokens: 64 us at 2, 76 at 4).  16 against 8 tiles a slice: one row over 777 tokens, one launch
 //   instead of two, 9.3 and 11.6 us.
 //   Many rows (4 tiles; 16 for heads over 128, whose partial results are twice as long: eight prompts of 313-364 tokens, 8 heads of
-//   256, 57 us uncut and 67 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
+//   256, 43 us uncut and 65 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
 //   7 / 1 heads of 64: 82 us uncut, 39 in slices).
 int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few, int min_tiles) {
     const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles * (few ? 1 : value_parts(kv.dim)), tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;

@@ -17,7 +17,7 @@
 //
 // A page scale that is no finite number, or (where a mask cuts the tile) a NaN code among the values, must not reach rows
 // that do not see the token, and 0 * NaN is NaN: such values are taken as zeros and the token's score becomes NaN for the
-// rows that see it.
+// rows that see it.  A key scale like that needs it as well: an infinite one makes scores of minus infinity, which weigh nothing.
 #pragma once
 #include <algorithm>
 #include "kvcache.hpp"
@@ -339,8 +339,8 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
             largest = __builtin_fmaxf(largest, x);
             reach(vsc, largest);
         }
-        const bool none = gp < 0, fine = finite(vs), more = tile + WAVES < tile_end;
         const float mul = ks * a.scale;
+        const bool none = gp < 0, fine = finite(vs) && finite(mul), more = tile + WAVES < tile_end;
         const bool odd = cut || __any(none || !fine);
         float sc[16];
 #pragma unroll
@@ -699,7 +699,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || RowType<T>::QP ==
         }
 #pragma unroll
         for (int u = 0; u < S; ++u) {
-            plain = plain && !__any(page[u] < 0 || !(ks[u] >= 0.f) || !finite(vs[u]) || vsc[u].factor != 1.f || out_of_reach(vsc[u], largest));
+            plain = plain && !__any(page[u] < 0 || !(ks[u] >= 0.f) || !finite(ks[u]) || !finite(vs[u]) || vsc[u].factor != 1.f || out_of_reach(vsc[u], largest));
         }
         f32x16 sc[2];
 #pragma unroll
@@ -779,7 +779,7 @@ static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || RowType<T>::QP ==
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int su = ONE ? 0 : u;
-                    const uint32_t bad = finite(vs[su]) ? bads[u] >> (16 * h2) : 0xffffu;
+                    const uint32_t bad = finite(ks[su]) && finite(vs[su]) ? bads[u] >> (16 * h2) : 0xffffu;
                     const int t0 = tok0 + u * 32 + h2 * 16;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {

@@ -575,8 +575,8 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * A row that sees no token gives zeros (lse: -infinity).  lse, if not NULL: [rows, q_heads] fp32, the natural logarithm of
  * the sum of exp(scale * q . k_j).  What tokens that a row does not see hold has no effect on it, NaN codes and scales of
  * pages without visible tokens included; a NaN among a visible token's values makes that dimension of the row, or the whole
- * row, NaN, and so does a scale of a visible token's page that is not finite.  dtype f32 f16 bf16 for q and out (which must
- * not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
+ * row, NaN, and so does a scale of a visible token's page that is not finite (key scales: times `scale`).  dtype f32 f16 bf16 for q and out
+ * (which must not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
  * queries enter the products exactly; a probability, together with its value scale, is rounded to f16, held relative to the
  * largest, for f16 and bf16 rows and kept to 22 bits for f32 rows.  A value scale enters as a power of two: |log2 scale| times
  * 2^-22 of relative error.  Values whose page's scale is below 2^-85 of the largest that the row sees, or below 2^-92, may lose

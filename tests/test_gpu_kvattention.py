@@ -360,6 +360,10 @@ def test_a_nan_among_values_reaches_only_rows_that_see_it(dxh, page, dim):
         c.v = keep
 
 
+def few(counts, lengths, extra=0):
+    return R.Rows(counts, lengths, extra=extra)
+
+
 # The host chooses the kernel by the rows that a sequence can have; with room for this many it is the one for many rows, whatever there is.
 def many(counts, lengths, extra=0):
     return R.Rows(counts, lengths, extra=extra, max_rows=1 << 15)
@@ -432,3 +436,29 @@ def test_value_scales_many(dxh, page, name):
         c.vs[:] = vs
         c.v[:] = 0 if vs == 0 else np.clip(c.v, -32, 32)
         check(dxh, c, many((40,), (9000,)), name, 1, size=0.0, far=121)
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code,page", [("i8", 16), ("e4m3", 64)])
+@pytest.mark.parametrize("room", [few, many], ids=["few", "many"])
+def test_a_scale_that_is_not_finite(dxh, room, code, page, name):
+    """a page whose key or value scale is an infinity or NaN, one token in it or all: rows that see it are NaN, whatever the sign of its products, the
+    others are as without it; of two key heads only its own is touched"""
+    for length, counts in ((page + 1, (3,)), (2 * page + 9, (page + 20,))):
+        c = R.Cache(code, page, 2, 64, 1, 3, seed=26)
+        rows = room(counts, (length,))
+        q = torch.rand(rows.rows, 4, 64, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") + 0.5
+        p = c.page_of(0, 1)
+        sees = torch.arange(length - counts[0], length) >= page
+        for sign in (1.0, -1.0):  # every product of the page's keys is of this sign
+            c.k[p] = R.encode(sign * (np.abs(R.decode(c.k[p], code)) + 1), 1, code)
+            clean = check(dxh, c, rows, name, 4, q=q)
+            for scales in (c.ks, c.vs):
+                keep = scales[p, 1]
+                for bad in (np.inf, -np.inf, np.nan):
+                    scales[p, 1] = bad
+                    out = torch.full_like(clean, 7.0)
+                    call(dxh, c.upload(), rows.upload(), name, q.to(R.TT[name]), out, None, 0.125, 1, 0)
+                    assert torch.equal(out[~sees], clean[~sees]) and torch.equal(out[sees][:, :2], clean[sees][:, :2]), (length, sign, bad)
+                    assert torch.isnan(out[sees][:, 2:]).all(), (length, sign, bad, scales is c.ks)
+                scales[p, 1] = keep

@@ -94,9 +94,14 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     a.scale = scale * kLog2e;
     a.causal = causal;
     a.window = window > INT32_MAX ? 0 : (int)window;
-    // A cache of twice the last-level cache is not in it from step to step: 1.2 GB of codes 227 us plain, 216 with nt loads (268 MB: 57
-    // and 62).  Several tiles of rows read the codes more than once.
-    a.nt = a.tile_rows == 16 && a.row_tiles == 1 && (int64_t)2 * a.kv.num_pages * a.kv.heads * a.kv.page_size * a.kv.dim > ((int64_t)512 << 20);
+    // Codes of a third more than the last-level cache are not in it from step to step, and reading them past it leaves it to what comes
+    // again (8 key heads of 128, 32 query heads, 1 to 32 sequences; plain against nt loads: 268 MB 49-50 and 51-54 us, 330 MB 60-66 and
+    // 60-69, 400 MB 75-82 and 71-77, 537 MB 104-110 and 91-103).  Pages of 128 keep plain loads: a tile reads half of a line of
+    // values, whose other half the next tile finds in the cache (268 MB 49 and 61 us, 819 MB 149 and 170).  What counts is the
+    // pages that the sequences can have, not the pool they are taken from: a server's pool is past any size.  Several tiles of
+    // rows read the codes more than once.
+    const int64_t pages = std::min<int64_t>(a.kv.num_pages, (int64_t)a.kv.batch * a.kv.pages_per_seq);
+    a.nt = a.tile_rows == 16 && a.row_tiles == 1 && a.kv.page_size == 64 && 2 * pages * a.kv.heads * a.kv.page_size * a.kv.dim > ((int64_t)340 << 20);
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + (size_t)a.splits * a.kv.rows * q_heads * a.kv.dim;
     hipStream_t st = as_stream(stream);

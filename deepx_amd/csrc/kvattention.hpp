@@ -34,7 +34,7 @@ struct AttArgs {
     float *lse, *part_o, *part_ml;  // partials: [slice][packed row][q head][dim] and [slice][packed row][q head][2]
     float scale;                    // scale * log2(e)
     int q_heads, group, causal, window, splits, min_tiles, row_tiles, tile_rows;
-    int nt;  // few rows and pages of at least 64 tokens: the codes are read past the last-level cache
+    int nt;  // few rows and pages of 64 tokens: the codes are read past the last-level cache
 };
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;

@@ -462,3 +462,26 @@ def test_a_scale_that_is_not_finite(dxh, room, code, page, name):
                     assert torch.equal(out[~sees], clean[~sees]) and torch.equal(out[sees][:, :2], clean[sees][:, :2]), (length, sign, bad)
                     assert torch.isnan(out[sees][:, 2:]).all(), (length, sign, bad, scales is c.ks)
                 scales[p, 1] = keep
+
+
+class PoolCache(R.Cache):
+    """The same cache at the start of a pool of `pool` bytes of keys: what a server allocates once."""
+    pool = 600 << 20
+
+    def upload(self):
+        pages = self.pool // (self.heads * self.page * self.dim)
+        self.dev = [torch.empty((pages, *t.shape[1:]), dtype=torch.from_numpy(t).dtype, device="cuda") for t in (self.k, self.v, self.ks, self.vs)]
+        for d, t in zip(self.dev, (self.k, self.v, self.ks, self.vs)):
+            d[:t.shape[0]] = torch.from_numpy(t).cuda()
+        self.dev_table = torch.from_numpy(self.table).cuda()
+        return dx.KvCache(*[t.data_ptr() for t in self.dev], self.dev_table.data_ptr(), pages, self.per_seq, self.page, self.heads, self.dim, R.CODE[self.code])
+
+
+@pytest.mark.parametrize("code,page,dim", [("i8", 64, 128), ("e4m3", 128, 64)])
+def test_the_pool_around_a_cache_changes_no_bit(dxh, code, page, dim):
+    """what serves a call goes by what its rows can read: the pages of their sequences, not the pool that those are taken from"""
+    args = (code, page, 2, dim, 2, 24)
+    rows = R.Rows((1, 2), (24 * page, 700))
+    for name in ("f32", "bf16"):
+        a, b = check(dxh, R.Cache(*args, seed=27), rows, name, 6), check(dxh, PoolCache(*args, seed=27), rows, name, 6)
+        assert torch.equal(a, b), name

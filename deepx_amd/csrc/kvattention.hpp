@@ -45,7 +45,9 @@ constexpr float kLift = 15.f;        // probabilities are held 2^15 times as lar
 // still at most 2^15.
 constexpr float kSlack = 8.f;
 // A row's sum of (2^15 times) p / v_scale, kept 2^-9 times as large, is finite for 2^30 tokens of the smallest scale, 2^-92 (what is
-// below is multiplied into the probabilities), and no less than 2^-123 for one token of the largest that fp32 values get, 2^121.
+// below is multiplied into the probabilities), and no less than 2^-123 for one token of the largest that written fp32 values get, 2^121.
+// Of a caller's own scales up to 2^128 the reciprocal and the sum can be subnormal (with 128-row tiles down to 2^-130, 19 bits): the hardware's
+// reciprocal and logarithm take them for zero and are given multiples of them (value_scale, lse_of).
 constexpr float kTinyScale = 0x1p-92f, kSumUnit = 0x1p-9f, kSumLog = 9.f;
 
 // ---- products ---------------------------------------------------------------------------------------------------------
@@ -140,7 +142,7 @@ struct ValueScale { float log, inv, factor; };
 __device__ __forceinline__ ValueScale value_scale(float vs) {
     if (!finite(vs)) vs = 1.f;
     const float mag = __builtin_fmaxf(__builtin_fabsf(vs), kTinyScale);
-    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag), __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p92f};
+    return {__builtin_amdgcn_logf(mag), __builtin_amdgcn_rcpf(mag * 0x1p-32f) * 0x1p-32f, __builtin_fabsf(vs) >= kTinyScale ? __builtin_copysignf(1.f, vs) : vs * 0x1p92f};
 }
 // Where a scale is so much smaller than the largest that the row has seen so far that 2^(t - m) could be 0 while the token's share of l is not (a page of
 // zeros beside one of huge values), the exponent keeps within kReach of that largest one's and the rest of the scale becomes a
@@ -230,7 +232,10 @@ template <typename T> __device__ __forceinline__ void store4(T *dst, float x0, f
     *reinterpret_cast<vec_t<T, 4> *>(dst) = w;
 }
 // `ref`: the power of two that l / kSumUnit and the output are counted in
-__device__ __forceinline__ float lse_of(float ref, float l) { return l == 0.f ? kNone : kLn2 * (ref + kSumLog + __builtin_amdgcn_logf(l)); }
+__device__ __forceinline__ float lse_of(float ref, float l) {
+    const bool small = l < 0x1p-100f;
+    return l == 0.f ? kNone : kLn2 * (ref + kSumLog + (small ? __builtin_amdgcn_logf(l * 0x1p64f) - 64.f : __builtin_amdgcn_logf(l)));
+}
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
 // One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its waves take the 64-token tiles in

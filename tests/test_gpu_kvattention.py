@@ -485,3 +485,16 @@ def test_the_pool_around_a_cache_changes_no_bit(dxh, code, page, dim):
     for name in ("f32", "bf16"):
         a, b = check(dxh, R.Cache(*args, seed=27), rows, name, 6), check(dxh, PoolCache(*args, seed=27), rows, name, 6)
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("room", [few, many], ids=["few", "many"])
+@pytest.mark.parametrize("code,page,dim,lengths", [("i8", 16, 64, (40,)), ("e4m3", 64, 128, (100, 3000)), ("i8", 128, 80, (9000,))], ids=str)
+def test_the_largest_value_scales(dxh, code, page, dim, lengths, room, name):
+    """scales up to the largest float under codes that keep the values finite: their reciprocals are less than any normal float"""
+    c = R.Cache(code, page, 1, dim, len(lengths), -(-max(lengths) // page), seed=28)
+    small = np.sign(R.decode(c.v, code)) / 4 * (4 if code == "i8" else 1)
+    c.v = R.encode(small * (np.random.default_rng(3).random(small.shape) < 0.5), 1, code)
+    for low, high in ((126.0, 127.9), (100.0, 127.9), (127.9, 127.9)):
+        c.vs = np.float32(2.0) ** np.random.default_rng(4).uniform(low, high, c.vs.shape).astype(np.float32)
+        check(dxh, c, room((2,) * len(lengths), lengths), name, 3, far=128)

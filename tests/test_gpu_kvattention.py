@@ -498,3 +498,49 @@ def test_the_largest_value_scales(dxh, code, page, dim, lengths, room, name):
     for low, high in ((126.0, 127.9), (100.0, 127.9), (127.9, 127.9)):
         c.vs = np.float32(2.0) ** np.random.default_rng(4).uniform(low, high, c.vs.shape).astype(np.float32)
         check(dxh, c, room((2,) * len(lengths), lengths), name, 3, far=128)
+
+
+def workgroups(L, c, rows, name, q_heads):
+    """of the kernel for few rows: the sequences' 16-row tiles of every key head, each as many times as the workspace holds partial results for"""
+    need = C.c_size_t(0)
+    dx.check(L.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], q_heads, C.byref(need)))
+    splits = max(1, round(need.value / (rows.rows * q_heads * (c.dim + 2) * 4)))
+    return len(rows.counts) * c.heads * -(-rows.max_rows * q_heads // c.heads // 16) * splits
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code,page,dim", [("i8", 16, 64), ("e4m3", 16, 128), ("e4m3", 32, 80), ("i8", 32, 128), ("i8", 64, 128), ("e4m3", 64, 64), ("i8", 128, 80), ("e4m3", 128, 128), ("i8", 64, 256), ("e4m3", 16, 192)])
+def test_batches_that_fill_the_card(dxh, code, page, dim, name):
+    """more workgroups than CUs, with sequences whose waves walk several tiles each: missing pages, windows that begin inside a tile, the worst codes
+    and scales where no row sees them, a NaN among the values of a late token"""
+    per = -(-1500 // page)
+    lengths = [1 + 487 * i % 1500 for i in range(38)] + [1500, 1490]
+    rows = R.Rows([1 + i % 2 for i in range(38)] + [2, 1], lengths, extra=1)
+    c = R.Cache(code, page, 4, dim, 40, per, seed=29, missing=[(0, 0, -1), (3, 0, 1 << 30), (38, 3, -1), (38, per - 2, -9), (39, 1, 1 << 30)])
+    assert workgroups(dxh, c, rows, name, 8) > 256
+    a = check(dxh, c, rows, name, 8)
+    assert torch.equal(a, check(dxh, c, rows, name, 8))
+    for window, causal in ((1000, 1), (333, 0)):
+        check(dxh, c, rows, name, 8, window=window, causal=causal)
+    seen = np.zeros((c.pages, page), bool)
+    for b, r, t in rows.each():
+        for slot in range(-(-(t + 1) // page) if t >= 0 else 0):
+            if c.page_of(b, slot) >= 0:
+                seen[c.page_of(b, slot), :min(page, t + 1 - slot * page)] = True
+    c.k[~np.broadcast_to(seen[:, None, :, None], c.k.shape)] = 127  # NaN in e4m3
+    c.v[~np.broadcast_to(seen[:, None, None, :], c.v.shape)] = 127
+    c.ks[~seen.any(1)] = np.nan
+    c.vs[~seen.any(1)] = np.inf
+    assert torch.equal(a, check(dxh, c, rows, name, 8))
+    if code == "e4m3":  # the last two tokens of the longest sequence: its first row sees one of them
+        first = int(rows.offsets[38])
+        c.v[c.page_of(38, 1498 // page), 1, 5, 1498 % page] = -1
+        c.v[c.page_of(38, 1499 // page), 2, 6, 1499 % page] = 127
+        out = torch.full_like(a, 7.0)
+        q = torch.randn(rows.rows, 8, dim, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(R.TT[name])
+        call(dxh, c.upload(), rows.upload(), name, q, out, None, dim ** -0.5, 1, 0)
+        assert torch.isnan(out[first:first + 2, 2:4, 5]).all() and torch.isnan(out[first + 1, 4:6, 6]).all()
+        same = torch.ones(rows.rows, 8, dtype=torch.bool, device="cuda")
+        same[first:first + 2, 2:4] = False
+        same[first + 1, 4:6] = False
+        assert torch.equal(out[same], a[same])

@@ -90,6 +90,12 @@ template <int LG> __device__ __forceinline__ float group_sum(float v) {
     if constexpr (LG >= 64) v += __shfl_xor(v, 32);
     return v;
 }
+// 1 / sqrt(v).  The hardware's takes a subnormal v (eps 0 over values below 2^-63) for zero: it gets 2^64 v.
+__device__ __forceinline__ float inv_sqrt(float v) {
+    const bool small = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v);
+    return small ? r * 0x1p32f : r;
+}
 // the value of lane ^ LG/2
 template <int LG> __device__ __forceinline__ float other_half(float v) {
     if constexpr (LG == 4) return dpp<kQuadXor2>(v);
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(kBlock) void normrope_kernel(const Args a) {
                 float sq = 0.f;
 #pragma unroll
                 for (int e = 0; e < V; ++e) sq = __builtin_fmaf(x[e], x[e], sq);
-                const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LG>(sq), inv_dim, a.eps));
+                const float r = inv_sqrt(__builtin_fmaf(group_sum<LG>(sq), inv_dim, a.eps));
 #pragma unroll
                 for (int e = 0; e < V; ++e) x[e] *= r * w[e];
             }
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(kBlock) void normrope_backward_kernel(const Args a)
                     sq = __builtin_fmaf(x[e], x[e], sq);
                     hx = __builtin_fmaf(g[e] * w[e], x[e], hx);
                 }
-                const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LG>(sq), inv_dim, a.eps));
+                const float r = inv_sqrt(__builtin_fmaf(group_sum<LG>(sq), inv_dim, a.eps));
                 const float q = group_sum<LG>(hx) * inv_dim * r * r;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {

@@ -232,3 +232,23 @@ def test_nothing_to_do(dxh):
     dx.check(dxh.dxh_normrope_backward(dx.F32, part, 1, 0, 64, 1e-6, None, ws.data_ptr(), ws.numel(), None))
     torch.cuda.synchronize()
     assert (dw == 0).all()  # the sum over no rows
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_squares_below_the_smallest_normal_float(dxh, name):
+    """eps 0 and heads whose mean square is subnormal: x^2 is exact to half of 2^-149, the mean of x = 2^-63 ... 2^-70 is 2^-126 ... 2^-140, so the sum is off by
+    at most a part in 2^9 there (2^-140 in steps of 2^-149) and the root by half of that; gradients: dx ~ 1 / |x| in fp32"""
+    dt, tt, et, _ = DT[name]
+    e = torch.arange(60, 71, dtype=torch.float32, device="cuda")
+    sign = torch.where(torch.arange(64, device="cuda") % 3 == 0, -1.0, 1.0)
+    x = (2.0 ** -e[:, None, None] * sign).to(tt)
+    y, dxv = torch.empty_like(x), torch.empty_like(x)
+    run_forward(dxh, dt, [x], [y], [None], dt, [1], 11, 64, 0.0, None)
+    assert ((y.float() - sign).abs() <= 2.0 ** -9 + et).all()
+    dy = torch.randn(11, 1, 64, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(tt)
+    dw, ws = torch.empty(64, device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    part = (dx.NormropePart * 1)(dx.NormropePart(heads(x), heads(dy), heads(dxv), None, dw.data_ptr(), 1, 1, dt))
+    dx.check(dxh.dxh_normrope_backward(dt, part, 1, 11, 64, 0.0, None, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    want, mag, dwant, dmag = ref_backward(x, dy, None, None, None, None, 0, False, 0.0, 1)
+    assert ((dxv.cpu().double() - want).abs() <= mag * 4 * 2.0 ** -9 + want.abs() * et).all()
+    assert ((dw.cpu().double() - dwant).abs() <= dmag * 2.0 ** -9).all()

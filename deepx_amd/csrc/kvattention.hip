@@ -16,7 +16,7 @@ namespace {
 bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
     if (rows <= (dtype == DXH_F32 ? 96 : 32)) return true;
     const int64_t tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64, pairs = (int64_t)kv.batch * kv.heads;
-    return 3 * pairs * ((rows + kTileRows - 1) / kTileRows) * value_parts(kv.dim) <= 2 * kCUs && pairs * ((rows + 15) / 16) * tiles <= 64 * kCUs;
+    return product(3, pairs, (rows + kTileRows - 1) / kTileRows, value_parts(kv.dim)) <= 2 * kCUs && product(pairs, (rows + 15) / 16, tiles) <= 64 * kCUs;
 }
 
 // How many slices the tokens of a sequence are cut into, counted on the longest sequence that the cache can hold; a slice has at
@@ -29,12 +29,12 @@ bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
 //   256, 43 us uncut and 65 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
 //   7 / 1 heads of 64: 82 us uncut, 39 in slices).
 int choose_splits(const KvArgs &kv, int q_heads, int64_t row_tiles, bool few, int min_tiles) {
-    const int64_t blocks = (int64_t)kv.batch * kv.heads * row_tiles * (few ? 1 : value_parts(kv.dim)), tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
+    const int64_t blocks = product(kv.batch, kv.heads, row_tiles, few ? 1 : value_parts(kv.dim)), tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64;
     int64_t want;
-    if (few) want = ((kv.batch > 1 ? 8 : 2) * kCUs + blocks - 1) / blocks;
-    else want = blocks < 2 * kCUs ? (4 * kCUs + blocks - 1) / blocks : 1;
+    if (few) want = ((kv.batch > 1 ? 8 : 2) * kCUs - 1) / blocks + 1;
+    else want = blocks < 2 * kCUs ? (4 * kCUs - 1) / blocks + 1 : 1;
     want = std::min<int64_t>(want, (tiles + min_tiles - 1) / min_tiles);
-    const int64_t row_bytes = kv.rows * q_heads * (kv.dim + 2) * 4;
+    const int64_t row_bytes = product(kv.rows, q_heads, (kv.dim + 2) * 4);
     want = std::min<int64_t>(want, ((int64_t)256 << 20) / std::max<int64_t>(1, row_bytes));  // partial results of at most 256 MiB
     return (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
 }
@@ -58,8 +58,8 @@ int plan(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, int32_t q_
     a.row_tiles = (int)((most + a.tile_rows - 1) / a.tile_rows);
     a.min_tiles = a.tile_rows == 16 || a.kv.dim > 128 ? 16 : 4;
     a.splits = choose_splits(a.kv, q_heads, a.row_tiles, a.tile_rows == 16, a.min_tiles);
-    const int64_t blocks = (int64_t)a.kv.batch * a.kv.heads * a.row_tiles * (a.tile_rows == 16 ? 1 : value_parts(a.kv.dim)), joins = a.splits > 1 ? (int64_t)a.kv.batch * a.kv.max_rows * q_heads : 0;
-    return launch_fits(blocks * a.splits, kBlock) && launch_fits(joins, kBlock) ? DXH_OK : DXH_ERR_TOO_LARGE;
+    const int64_t blocks = product(a.kv.batch, a.kv.heads, a.row_tiles, a.tile_rows == 16 ? 1 : value_parts(a.kv.dim), a.splits), joins = a.splits > 1 ? product(a.kv.batch, a.kv.max_rows, q_heads) : 0;
+    return launch_fits(blocks, kBlock) && launch_fits(joins, kBlock) ? DXH_OK : DXH_ERR_TOO_LARGE;
 }
 
 }  // namespace
@@ -101,7 +101,7 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     // pages that the sequences can have, not the pool they are taken from: a server's pool is past any size.  Several tiles of
     // rows read the codes more than once.
     const int64_t pages = std::min<int64_t>(a.kv.num_pages, (int64_t)a.kv.batch * a.kv.pages_per_seq);
-    a.nt = a.tile_rows == 16 && a.row_tiles == 1 && a.kv.page_size == 64 && 2 * pages * a.kv.heads * a.kv.page_size * a.kv.dim > ((int64_t)340 << 20);
+    a.nt = a.tile_rows == 16 && a.row_tiles == 1 && a.kv.page_size == 64 && product(2 * pages, a.kv.heads, a.kv.page_size, a.kv.dim) > ((int64_t)340 << 20);
     a.part_o = (float *)workspace;
     a.part_ml = a.part_o + (size_t)a.splits * a.kv.rows * q_heads * a.kv.dim;
     hipStream_t st = as_stream(stream);

@@ -280,7 +280,7 @@ __global__ __launch_bounds__(THREADS) void kvcache_read_kernel(const RowsArgs a)
 }
 
 template <typename T, typename Code> int launch(const RowsArgs &a, bool write, hipStream_t st) {
-    const int64_t blocks = (int64_t)2 * a.kv.heads * a.slots * a.kv.batch;
+    const int64_t blocks = product(2, a.kv.heads, a.slots, a.kv.batch);
     // a lane for every 16 codes of a page, as one new row can change the scale of all: one wave or four
     const bool wide = a.kv.page_size * a.kv.dim > 16 * kWave;
     if (!launch_fits(blocks, wide ? 256 : 64)) return DXH_ERR_TOO_LARGE;
@@ -311,7 +311,7 @@ int rows_call(const dxh_kvcache *cache, const dxh_kvrows *rows, int dtype, const
     if (!write && a.data[0] == a.data[1]) return DXH_ERR_ARG;  // two results in one place
     // n rows that start anywhere in a page touch at most this many
     a.slots = (int)(((int64_t)a.kv.max_rows + a.kv.page_size - 2) / a.kv.page_size) + 1;
-    a.nt = use_nt_store((size_t)2 * a.kv.rows * a.kv.heads * a.kv.dim * dtype_size(dtype));
+    a.nt = use_nt_store((size_t)product(2 * a.kv.rows, a.kv.heads, a.kv.dim * dtype_size(dtype)));
     hipStream_t st = as_stream(stream);
     const bool i8 = cache->code == DXH_I8;
     switch (dtype) {

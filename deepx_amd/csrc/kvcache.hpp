@@ -105,8 +105,14 @@ inline int kv_check(const dxh_kvcache *c, const dxh_kvrows *r, int dtype, KvArgs
     if (c->num_pages > 0 && c->pages_per_seq > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale || c->k == c->v || c->k_scale == c->v_scale)) return DXH_ERR_ARG;
     return DXH_OK;
 }
+// The product of counts that are each at most 2^63 - 1, or 2^63 - 1 if that is less
+inline int64_t product(int64_t a) { return a; }
+template <typename... More> int64_t product(int64_t a, int64_t b, More... more) {
+    int64_t p;
+    return product(__builtin_mul_overflow(a, b, &p) ? (a && b ? INT64_MAX : 0) : p, more...);
+}
 // a launch has fewer than 2^32 work items
-inline bool launch_fits(int64_t blocks, int threads) { return blocks * threads <= (int64_t)UINT32_MAX; }
+inline bool launch_fits(int64_t blocks, int threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
 inline bool kv_nothing(const KvArgs &a) { return a.batch == 0 || a.rows == 0 || a.max_rows == 0; }
 inline int kv_heads_check(const dxh_heads *h, int es, bool used) {
     if (!h || (used && !h->data)) return DXH_ERR_ARG;

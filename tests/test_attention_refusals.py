@@ -166,3 +166,16 @@ def test_sizes_past_one_launch():
     assert L.dxh_kvcache_write(cache(), rows, dx.BF16, heads(), heads(16384), None) == big  # 2^23 sequences, 2 heads, keys and values, 2 pages each, 64 lanes
     assert L.dxh_kvcache_attention_workspace_bytes(cache(), kvrows(rows=1 << 24, batch=1 << 23, max_rows=1), dx.BF16, 14, C.byref(n)) == big
     assert L.dxh_kvcache_attention(cache(), kvrows(rows=1), dx.BF16, 14, heads(), heads(8192), None, 3e38, 1, 0, None, 0, None) == ARG
+
+
+def test_counts_whose_products_pass_64_bits():
+    """sizes that are each within their limits but not together: too large, not wrapped around into a launch that fits"""
+    L, big, top = dx.load(), -6, (1 << 31) - 1
+    n = C.c_size_t(1)
+    # the second writes 2 x 2^30 heads x (2^27 + 1) slots x 2^30 sequences: of 2^88 + 2^61 workgroups of 64 lanes, none is left in 64 bits
+    for heads_, batch, most in ((1 << 26, 1 << 10, top), (1 << 30, 1 << 30, top), (top, top, top), (1 << 20, 1 << 24, 1 << 24)):
+        c, r = cache(heads=heads_, pages_per_seq=1), kvrows(rows=1, batch=batch, max_rows=most)
+        for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
+            assert fn(c, r, dx.BF16, heads(), heads(16384), None) == big, (heads_, batch, most)
+        for q in (heads_, top // heads_ * heads_):
+            assert L.dxh_kvcache_attention_workspace_bytes(c, r, dx.BF16, q, C.byref(n)) == big, (heads_, batch, most)

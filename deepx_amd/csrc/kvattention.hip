@@ -88,6 +88,7 @@ int dxh_kvcache_attention(const dxh_kvcache *cache, const dxh_kvrows *rows, int 
     if (q->data == out->data) return DXH_ERR_ARG;  // a row's queries are read by several workgroups
     const size_t need = part_bytes(a.kv, q_heads, a.splits);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return DXH_ERR_WORKSPACE;
+    if (kv_meets(a.kv, out->data) || kv_meets(a.kv, lse) || (lse && (lse == out->data || lse == q->data))) return DXH_ERR_ARG;
     a.q = (const char *)q->data; a.q_row = q->row_stride; a.q_head = q->head_stride;
     a.out = (char *)out->data; a.o_row = out->row_stride; a.o_head = out->head_stride;
     a.lse = lse;

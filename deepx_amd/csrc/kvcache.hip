@@ -284,6 +284,7 @@ template <typename T, typename Code> int launch(const RowsArgs &a, bool write, h
     // a lane for every 16 codes of a page, as one new row can change the scale of all: one wave or four
     const bool wide = a.kv.page_size * a.kv.dim > 16 * kWave;
     if (!launch_fits(blocks, wide ? 256 : 64)) return DXH_ERR_TOO_LARGE;
+    if (kv_meets(a.kv, a.data[0]) || kv_meets(a.kv, a.data[1])) return DXH_ERR_ARG;
     if (write) {
         if (wide) kvcache_write_kernel<T, Code, 256><<<(unsigned)blocks, 256, 0, st>>>(a);
         else kvcache_write_kernel<T, Code, 64><<<(unsigned)blocks, 64, 0, st>>>(a);

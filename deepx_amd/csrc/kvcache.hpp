@@ -113,6 +113,10 @@ template <typename... More> int64_t product(int64_t a, int64_t b, More... more) 
 }
 // a launch has fewer than 2^32 work items
 inline bool launch_fits(int64_t blocks, int threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
+// does what a call writes, or writes into the cache, begin where something else that it reads or writes does
+inline bool kv_meets(const KvArgs &a, const void *p) {
+    return p && (p == a.k || p == a.v || p == a.k_scale || p == a.v_scale || p == a.table || p == a.offsets || p == a.lengths);
+}
 inline bool kv_nothing(const KvArgs &a) { return a.batch == 0 || a.rows == 0 || a.max_rows == 0; }
 inline int kv_heads_check(const dxh_heads *h, int es, bool used) {
     if (!h || (used && !h->data)) return DXH_ERR_ARG;

@@ -353,7 +353,10 @@ int check(int dtype, const dxh_normrope_part *parts, int nparts, int64_t rows, i
     for (int i = 0; i < nparts; ++i)
         for (int j = 0; j < nparts; ++j) {
             const Part &p = a.part[i], &q = a.part[j];
-            if (i == j || rows == 0 || !p.heads || !q.heads) continue;
+            if (rows == 0 || !p.heads) continue;
+            if ((q.w && p.out == q.w) || (a.rd && (p.out == a.cos || p.out == a.sin || (a.positions && p.out == a.positions)))) return DXH_ERR_ARG;
+            if (q.dw && p.out == q.dw) return DXH_ERR_ARG;
+            if (i == j || !q.heads) continue;
             if (p.out == q.out || p.out == q.x || (back && p.out == q.y_in)) return DXH_ERR_ARG;
             if (p.dw && p.dw == q.dw) return DXH_ERR_ARG;
         }

@@ -495,7 +495,8 @@ typedef struct dxh_heads {
  *   the other values of the head pass unchanged.
  * Computed in fp32, one rounding of the result.  cos / sin: fp32 [table_rows, rotary.dim / 2]; a position outside the table
  * is clamped into it; positions NULL: 0, 1, 2 ...  rotary NULL or rotary.dim = 0: no rotation.  y may be x itself (the same
- * pointer and strides); any other overlap is not allowed.  dtypes f32 f16 bf16, weights of the same dtype or f32, dim a
+ * pointer and strides); any other overlap is not allowed, and DXH_ERR_ARG where a result begins in the place of another result, a
+ * weight, a table or another part's input.  dtypes f32 f16 bf16, weights of the same dtype or f32, dim a
  * multiple of 16 up to 256, rotary.dim any even number up to dim. */
 #define DXH_NORMROPE_MAX_PARTS 4
 typedef struct dxh_rotary {
@@ -542,7 +543,8 @@ DXH_API int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int
  * has no place in the cache: it is not written and reads as zeros.  Rows of a sequence beyond max_rows and rows behind the
  * last sequence are left as they are; offsets outside [0, rows] are clamped into it: no content of the device arrays makes
  * a call touch memory outside its tensors.
- * Nothing of the device arrays is read on the host, so a recorded graph follows them as they change. */
+ * Nothing of the device arrays is read on the host, so a recorded graph follows them as they change.  Rows, results and the cache
+ * must not overlap; DXH_ERR_ARG where one begins in the place of another. */
 typedef struct dxh_kvcache {
     void *k, *v;
     float *k_scale, *v_scale;

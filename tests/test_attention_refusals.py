@@ -179,3 +179,28 @@ def test_counts_whose_products_pass_64_bits():
             assert fn(c, r, dx.BF16, heads(), heads(16384), None) == big, (heads_, batch, most)
         for q in (heads_, top // heads_ * heads_):
             assert L.dxh_kvcache_attention_workspace_bytes(c, r, dx.BF16, q, C.byref(n)) == big, (heads_, batch, most)
+
+
+def test_results_in_the_place_of_weights_tables_scales_and_each_other():
+    L = dx.load()
+    fwd = lambda *parts: L.dxh_normrope(dx.BF16, (dx.NormropePart * len(parts))(*parts), len(parts), 1, 64, 1e-6, rotary(), None)  # noqa: E731
+    other = norm_part(x=heads(32768), y=heads(40960), weight=49152)
+    for part in (norm_part(y=heads(256)), norm_part(y=heads(49152)), norm_part(y=heads(512)), norm_part(y=heads(1024))):  # its weight, the other's, sines, positions
+        assert fwd(part, other) == ARG and fwd(other, part) == ARG
+    assert fwd(norm_part(y=heads(256), weight=2048, norm=0)) == ARG  # cosines
+    other = norm_part(x=heads(32768), y=heads(40960), dx=heads(57344), weight=49152, dweight=65536)
+    back = lambda *parts: L.dxh_normrope_backward(dx.F32, (dx.NormropePart * len(parts))(*parts), len(parts), 1, 64, 1e-6, rotary(positions=None), 1 << 20, 1 << 30, None)  # noqa: E731
+    for part in (norm_part(dx=heads(49152)), norm_part(dx=heads(65536)), norm_part(dweight=57344), norm_part(dweight=16384)):
+        part.weight_dtype = other.weight_dtype = dx.F32
+        assert back(part, other) == ARG and back(other, part) == ARG
+    rows = kvrows(rows=1)
+    for lse in (4096, 12288, 8192 + 16384, 256, 512, 1024, 256 * 3):
+        assert L.dxh_kvcache_attention(cache(v=12288, k=24576), kvrows(rows=1, lengths=768), dx.BF16, 14, heads(4096), heads(8192), lse, 0.125, 1, 0, None, 0, None) == ARG, lse
+    assert L.dxh_kvcache_attention(cache(), rows, dx.BF16, 14, heads(16384), heads(32768), 32768, 0.125, 1, 0, None, 0, None) == ARG
+    for out in (4096, 8192):  # the codes
+        assert L.dxh_kvcache_attention(cache(), rows, dx.BF16, 14, heads(16384), heads(out), None, 0.125, 1, 0, None, 0, None) == ARG
+        for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
+            assert fn(cache(), rows, dx.BF16, heads(out), heads(16384), None) == ARG and fn(cache(), rows, dx.BF16, heads(16384), heads(out), None) == ARG
+    for out in (256, 512, 1024):  # scales and offsets, the page table
+        for fn in (L.dxh_kvcache_write, L.dxh_kvcache_read):
+            assert fn(cache(), rows, dx.BF16, heads(16384), heads(out), None) == ARG

@@ -234,3 +234,25 @@ def test_lines_that_are_refused(tmp_path):
         assert not h.get("o").any()  # no sequence has rows: offsets are zeros
     finally:
         ex.close()
+
+
+def test_results_that_are_other_inputs_are_refused(tmp_path):
+    """a line whose result is also its weight, another part's, a gradient's other result or a scale of the cache"""
+    ex = InProc()
+    try:
+        h = Host(ex, tmp_path)
+        for name, shape, dt in (("x", [1, 1, 64], "float32"), ("x2", [1, 1, 64], "float32"), ("w", [1, 1, 64], "float32"), ("w2", [64], "float32"), ("g", [1, 1, 64], "float32"), ("y", [1, 1, 64], "float32"),
+                                ("cos", [8, 32], "float32"), ("sin", [8, 32], "float32"), ("pos", [1], "int32"), ("q", [4, 2, 64], "float32"), ("o", [4, 2, 64], "float32"), ("kc", [4, 2, 16, 64], "int8"),
+                                ("vc", [4, 2, 64, 16], "int8"), ("ks", [4, 2], "float32"), ("vs", [4, 2], "float32"), ("off", [3], "int32"), ("len", [2], "int32"), ("table", [2, 2], "int32")):
+            h.run(f"newtensor(vector<int32>:[{' '.join(map(str, shape))}])->(tensor<{dt}>:{name})")
+        tab = "tensor<float32>:cos, tensor<float32>:sin, tensor<int32>:pos, var<float32>:1e-6, var<bool>:false"
+        nr = lambda xs, ws, ys: f"normrope(listtensor<any>:[{xs}], listtensor<any>:[{ws}], {tab})->(listtensor<any>:[{ys}])"  # noqa: E731
+        back = lambda dxs, dws: f"normropebackward(listtensor<any>:[x], listtensor<any>:[g], listtensor<any>:[w], {tab})->(listtensor<any>:[{dxs}], listtensor<any>:[{dws}])"  # noqa: E731
+        at = lambda lse: ("kvcacheattention(tensor<any>:q, listtensor<any>:[kc vc ks vs], tensor<int32>:off, tensor<int32>:len, tensor<int32>:table, var<int32>:2, var<float32>:0.1, var<bool>:true, var<int32>:0, "  # noqa: E731
+                          f"var<string>:int8)->(tensor<any>:o, tensor<float32>:{lse})")
+        for line in (nr("x", "w", "w"), nr("x x2", "w w2", "y w"), back("w", "w2"), back("y", "y"), at("ks"), at("vs")):
+            assert " error//" in ex.execute(line), line
+        h.run(nr("x x2", "w w2", "x y"))
+        h.run(back("g", "w2"))
+    finally:
+        ex.close()

@@ -4,11 +4,17 @@
 // query row i and head g of the G that share the key head.  With codes K', V' and page scales k_s, v_s, in base 2:
 //     s_j = (Q K'^T)_j k_s(j) scale log2(e),     t_j = s_j + log2 v_s(j),     m = max t_j,     p_j = 2^(t_j - m),
 //     O   = sum p_j V'_j,     l = sum p_j / v_s(j),     out = O / l,     lse = ln 2 (m + log2 l).
-// Taking the value scale into the exponent keeps p in (0, 1] whatever the scales are, so that it can be rounded to f16 (held
-// 2^15 times as large, or 2^7 times with 128-row tiles: normal down to 2^-29 or 2^-21 of the largest): 2^-11 of a term where bf16 would lose 2^-8, on the same matrix
-// instruction.  Codes are whole numbers below 2^8 or e4m3 values, exact in bf16 and in f16, and enter the products
-// exactly; scales are applied to scores in fp32.  Q is exact too: bf16 rows multiply bf16 keys, f16 rows f16 keys; f32 rows are split
-// into three bf16 parts (24 bits) and their p into two f16 parts, each part one more product.
+// Taking the value scale into the exponent keeps p in (0, 1] whatever the scales are, so that it can be rounded to f16 (held 2^15 times
+// as large, or 2^7 times with 128-row tiles of 16-bit rows: normal down to 2^-29 or 2^-21 of the largest): 2^-11 of a term where bf16
+// would lose 2^-8, on the same matrix instruction.  Codes are whole numbers below 2^8 or e4m3 values, exact in bf16 and in f16, and
+// enter the products exactly; scales are applied to scores in fp32.  Q is exact too: bf16 rows multiply bf16 keys, f16 rows f16 keys;
+// f32 rows are split into three bf16 parts (24 bits).
+//
+// A probability is held in two f16 parts, 22 bits, each one more product, but for 16-bit rows in the kernel for many rows.  There the
+// second part costs a quarter of the time (four prompts of 3.3k-4.1k tokens, 32 / 8 heads of 128: 652 and 831 us), and bf16 results are
+// 1.67e-3 from the exact value with one part, 1.66e-3 with two, which is their own rounding (f16: 2.8e-4 and 2.1e-4).  Under few rows it
+// hides behind the codes' loads, 64 rows over 1k-16k tokens 213 us with one and 212 with two, f16 results 2.5e-4 and 2.1e-4 from the exact
+// value; where the codes stay in the caches it costs 2 - 6 % (4 x 8 rows over 3k-6k tokens, 24 / 4 heads of 128: 24.3 and 25.2 us).
 //
 // Everything is computed transposed, S^T = K' Q^T and O^T = V'^T P^T, so that the tokens of a score tile are rows of the
 // accumulator and a probability is already in the lane that feeds it to the second product: no exchange between lanes.
@@ -51,7 +57,7 @@ constexpr float kSlack = 8.f;
 constexpr float kTinyScale = 0x1p-92f, kSumUnit = 0x1p-9f, kSumLog = 9.f;
 
 // ---- products ---------------------------------------------------------------------------------------------------------
-// Kind: the 16-bit type of keys and queries; QP, PP: parts that hold a query value, a probability
+// Kind: the 16-bit type of keys and queries; QP, PP: parts that hold a query value, a probability of the kernel for many rows
 template <typename T> struct RowType { using Kind = __bf16; static constexpr int QP = 1, PP = 1; };
 template <> struct RowType<f16_t> { using Kind = _Float16; static constexpr int QP = 1, PP = 1; };
 template <> struct RowType<float> { using Kind = __bf16; static constexpr int QP = 3, PP = 2; };
@@ -245,7 +251,7 @@ __device__ __forceinline__ float lse_of(float ref, float l) {
 template <typename T, typename Code, int SPANS, bool EXACT, bool ONE, bool NT, int WAVES>
 static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 1 : SPANS == 2 || RowType<T>::QP > 1 ? 2 : 3) void kvattention_rows_kernel(const AttArgs a) {
     using Kind = typename RowType<T>::Kind;
-    constexpr int QP = RowType<T>::QP, PP = RowType<T>::PP, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
+    constexpr int QP = RowType<T>::QP, PP = 2, DT = SPANS * 4;  // DT: 16-dimension tiles of the padded head
     __shared__ float meet_o[WAVES / 2][16][SPANS * 64 + 4];
     __shared__ float meet_m[WAVES][16], meet_l[WAVES][16];
     unsigned blk = blockIdx.x;

@@ -579,8 +579,9 @@ DXH_API int dxh_kvcache_read(const dxh_kvcache *cache, const dxh_kvrows *rows, i
  * pages without visible tokens included; a NaN among a visible token's values makes that dimension of the row, or the whole
  * row, NaN, and so does a scale of a visible token's page that is not finite (key scales: times `scale`).  dtype f32 f16 bf16 for q and out
  * (which must not overlap); q_heads a multiple of cache->heads.  Scores, maxima, sums and the output are accumulated in fp32; codes and
- * queries enter the products exactly; a probability, together with its value scale, is rounded to f16, held relative to the
- * largest, for f16 and bf16 rows and kept to 22 bits for f32 rows.  A value scale enters as a power of two: |log2 scale| times
+ * queries enter the products exactly; a probability, together with its value scale and relative to the largest, is kept to 22 bits, but
+ * rounded to f16 (a relative 2^-11) for f16 and bf16 rows where the kernel for many rows serves the call: max_rows * q_heads / heads over
+ * 32, unless that is little work.  A value scale enters as a power of two: |log2 scale| times
  * 2^-22 of relative error.  Values whose page's scale is below 2^-85 of the largest that the row sees, or below 2^-92, may lose
  * precision down to zeros; queries times codes summed over a head must stay finite in fp32.
  * A long cache under few rows is cut into slices whose partial results lie in `workspace` and are joined in slice order by a

@@ -544,3 +544,18 @@ def test_batches_that_fill_the_card(dxh, code, page, dim, name):
         same[first:first + 2, 2:4] = False
         same[first + 1, 4:6] = False
         assert torch.equal(out[same], a[same])
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("code,page,dim,counts,lengths", [("i8", 16, 64, (1,), (777,)), ("e4m3", 64, 128, (1, 4, 2), (3000, 500, 64)), ("i8", 128, 80, (4,), (9000,)), ("e4m3", 32, 256, (3, 1), (900, 70))], ids=str)
+def test_probabilities_of_few_rows_keep_22_bits(dxh, code, page, dim, counts, lengths, name):
+    """16-bit rows differ from the 64-bit value by what f32 rows may, and by one rounding of the result"""
+    c = R.Cache(code, page, 2, dim, len(counts), -(-max(lengths) // page), seed=30)
+    rows = R.Rows(counts, lengths)
+    q = torch.randn(rows.rows, 6, dim, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(R.TT[name])
+    out = torch.empty_like(q)
+    call(dxh, c.upload(), rows.upload(), name, q, out, None, dim ** -0.5, 1, 0)
+    for r, entry in R.attention(c, rows, q.double().cpu().numpy(), dim ** -0.5, 1, 0).items():
+        bar = R.attention_bar("f32", c, entry)[0] + np.abs(entry[0]) * R.HALF_STEP[name] * (1 + 2 ** -8) + R.TINY[name]
+        worst = float((np.abs(out[r].double().cpu().numpy() - entry[0]) / bar).max())
+        assert worst <= 1, (r, worst)

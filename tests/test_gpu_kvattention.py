@@ -559,3 +559,52 @@ def test_probabilities_of_few_rows_keep_22_bits(dxh, code, page, dim, counts, le
         bar = R.attention_bar("f32", c, entry)[0] + np.abs(entry[0]) * R.HALF_STEP[name] * (1 + 2 ** -8) + R.TINY[name]
         worst = float((np.abs(out[r].double().cpu().numpy() - entry[0]) / bar).max())
         assert worst <= 1, (r, worst)
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_what_eight_bits_cost(dxh, code):
+    """A prompt and then tokens one by one, keys five times the size of the rest: what is read back against what was written, and the attention over the
+    cache against the 64-bit attention over keys and values as they were.  With s a page's scale in the end:
+      int8: a code is off by s / 2, and by as much again each time its page grew, at scales of at most s; an fp32 product by 2^-24 of 127 s;
+      e4m3: by 2^-4 of the value and 2^-10 s (half its smallest step, 2^-9), each time relative to what the code was before;
+      attention: scores off by e = scale sum |q| dk move weights by at most exp(2 e), values by dv: |out' - out| <= max dv + (exp(2 e) - 1) sum p |v|."""
+    hq, hk, dim, page = 6, 2, 64, 16
+    c = R.Cache(code, page, hk, dim, 2, 8, seed=31)
+    cache = c.upload()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    have, kept, writes = [0, 0], [[[], []], [[], []]], np.zeros((2, 8), int)
+    for counts in ((37, 80), (1, 1), (1, 1), (2, 0), (1, 3)):
+        have = [a + b for a, b in zip(have, counts)]
+        rows = R.Rows(counts, have)
+        desc = rows.upload()
+        q, k, v = (torch.randn(rows.rows, h, dim, generator=g, device="cuda") * size for h, size in ((hq, 0.3), (hk, 5.0), (hk, 1.0)))
+        dx.check(dxh.dxh_kvcache_write(cache, desc, dx.F32, R.heads(k), R.heads(v), stream()))
+        out, back = torch.empty_like(q), [torch.empty_like(k), torch.empty_like(v)]
+        call(dxh, cache, desc, "f32", q, out, None, dim ** -0.5, 1, 0)
+        dx.check(dxh.dxh_kvcache_read(cache, desc, dx.F32, R.heads(back[0]), R.heads(back[1]), stream()))
+        c.k, c.v, c.ks, c.vs = c.download()
+        for b, r, t in rows.each():
+            for i, x in enumerate((k, v)):
+                kept[b][i].append(x[r].double().cpu().numpy())
+        for b in range(2):
+            for slot in {t // page for bb, _, t in rows.each() if bb == b}:
+                writes[b, slot] += 1
+        off = lambda x, s, n: (n * s / 2 + s * 127 * 2 ** -23 if code == "i8" else np.abs(x) * ((1 + 2 ** -4) ** n - 1) * (1 + 2 ** -20) + n * (s * 2 ** -10) * (1 + 2 ** -4) ** n)  # noqa: E731
+        got = [t.double().cpu().numpy() for t in back]
+        for b, r, t in rows.each():
+            for i, scales in enumerate((c.ks, c.vs)):
+                x, s = kept[b][i][t], scales[c.page_of(b, t // page)].astype(np.float64)[:, None]
+                assert (np.abs(got[i][r] - x) <= off(x, s, 1)).all(), (b, t, i)
+        for b, r, t in rows.each():
+            K, V = (np.stack(kept[b][i][:t + 1]) for i in (0, 1))
+            pages, n = [c.page_of(b, j // page) for j in range(t + 1)], np.array([writes[b, j // page] for j in range(t + 1)])[:, None, None]
+            dk, dv = off(K, c.ks[pages].astype(np.float64)[..., None], n), off(V, c.vs[pages].astype(np.float64)[..., None], n)
+            for h in range(hq):
+                qq, kh = q[r, h].double().cpu().numpy(), h // (hq // hk)
+                s = K[:, kh] @ qq * dim ** -0.5
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                e = (np.abs(qq) * np.broadcast_to(dk[:, kh], K[:, kh].shape)).sum(1).max() * dim ** -0.5
+                bar = np.broadcast_to(dv[:, kh], V[:, kh].shape).max(0) + (np.exp(2 * e) - 1) * (p @ np.abs(V[:, kh])) + 1e-5
+                err = np.abs(out[r, h].double().cpu().numpy() - p @ V[:, kh])
+                assert (err <= bar).all(), (b, t, h, float((err / bar).max()))

@@ -8,11 +8,13 @@ namespace {
 // Which of the two kernels; `rows` of one sequence and key head.  The 16-row kernel decodes a tile of codes for every 16 rows, the other for
 // every 128, but padded to that many rows and a tile at a time behind two barriers.  16-row against 128-row kernel, bf16 unless said:
 //   up to 32 rows always; up to 96 f32 rows, whose products cost more than the codes (48 rows over 3k-8k tokens, 16 x 4 heads of
-//   128: 64 and 122 us; bf16, 35 rows over 4k-8k, 16 x 8 heads: 101 and 93);
+//   128: 64 and 122 us; bf16, 35 rows over 4k-8k, 16 x 8 heads: 103 and 91);
 //   else where the 128-row tiles leave a third of the CUs idle and there is little work, at most 64 products of a 16-row and a 64-token tile a CU: a prompt
-//   of 512 tokens, 16 / 4 heads of 128, 13.0 and 23.4; a prompt of 300, f32, 2 / 1 heads of 80, 9.7 and 25.6; but four f32 prompts of
+//   of 512 tokens, 16 / 4 heads of 128, 13.6 and 23.2; a prompt of 300, f32, 2 / 1 heads of 80, 9.7 and 25.7; but four f32 prompts of
 //   2000, 8 / 2 heads of 128 (128 products a CU), 132 and 114, and eight prompts of 128, 32 / 8 heads of 128 (as many 128-row tiles as
-//   CUs), 29.8 and 14.7; eight of 313-364, 8 heads of 256, 77 and 43.
+//   CUs), 31 and 14.5; eight of 313-364, 8 heads of 256, 75 and 34.
+// Tiles of tokens are those that the table has room for, as the host does not see the lengths: a table much wider than its sequences
+// can send a short prompt to the kernel for many rows.
 bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
     if (rows <= (dtype == DXH_F32 ? 96 : 32)) return true;
     const int64_t tiles = ((int64_t)kv.pages_per_seq * kv.page_size + 63) / 64, pairs = (int64_t)kv.batch * kv.heads;
@@ -24,7 +26,7 @@ bool few_rows(const KvArgs &kv, int64_t rows, int dtype) {
 //   Few rows (16 tiles a slice): the sequences of a batch differ in length, and 8 workgroups a CU let the card fill the gaps that
 //   short ones leave (64 sequences of 1k-16k tokens: 245 us at 4, 229 at 8, 230 at 16); one sequence is cut into what runs at once,
 //   two workgroups a CU (131071 tokens: 64 us at 2, 76 at 4).  16 against 8 tiles a slice: one row over 777 tokens, one launch
-//   instead of two, 9.3 and 11.6 us.
+//   instead of two, 9.7 and 12.8 us.
 //   Many rows (4 tiles; 16 for heads over 128, whose partial results are twice as long: eight prompts of 313-364 tokens, 8 heads of
 //   256, 43 us uncut and 65 in two slices): only where the tiles of rows alone leave CUs idle (two prompts of 1832 and 498 tokens,
 //   7 / 1 heads of 64: 82 us uncut, 39 in slices).

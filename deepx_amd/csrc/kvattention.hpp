@@ -245,7 +245,7 @@ __device__ __forceinline__ float lse_of(float ref, float l) {
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
 // One workgroup: 16 rows of one (sequence, key head), one slice of the tokens; its waves take the 64-token tiles in
-// turn and meet at the end (four waves; eight where there is at most a workgroup a CU: one row over 777 tokens 9.0 -> 8.6 us).  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
+// turn and meet at the end (four waves; eight where there is at most a workgroup a CU: one row over 777 tokens 9.5 -> 8.9 us).  Row 4g + r of 16-token score tile t is token 16g + 4t + r: lane group g holds tokens 16g .. 16g + 15,
 // loads codes straight into the operands' registers (no LDS) and needs one page and one scale.  Bound by the bytes of the codes:
 // 64 rows over 1k-16k tokens, 32 / 8 heads of 128 in e4m3, 211 us (5.5 TB/s); 4 rows over 131071 in int8, 53 us (5.0 TB/s).
 template <typename T, typename Code, int SPANS, bool EXACT, bool ONE, bool NT, int WAVES>
@@ -481,13 +481,16 @@ static __global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? 2 : SPANS == 4 ? 
 // row 8b + 4h + r of one is token 16h + 4b + r, so lane half h holds 16 consecutive tokens of one page and feeds
 // their probabilities to the second product as they are.  Rows of LDS are padded by 16 bytes: 16 lanes that read 16 bytes at
 // one column of 16 rows meet 16 different bank groups.
-// Bound by the vector pipe and what it cannot hide: causal prompts of 4 x 3.3k-4.1k tokens, 32 / 8 heads of 128, 640 us (760
-// TFLOP/s), matrix pipe busy 31 %, vector pipe 45 % (2^x a third of that), waves waiting 34 %.  Eight waves a workgroup, two
+// Bound by the vector pipe and what it cannot hide: causal prompts of 4 x 3.3k-4.1k tokens, 32 / 8 heads of 128, 636 us (765
+// TFLOP/s), matrix pipe busy 31 %, vector pipe 48 % (2^x a third of that), waves waiting 29 %; 1.3 LDS instructions a product, whose bank
+// conflicts add 0.8 cycles each.  Eight waves a workgroup, two
 // buffers with one barrier a tile, an enforced alternation of matrix and vector instructions, and raised wave priority under
 // the products were measured at 682, 672, 669 and 674 us.
 // Heads over 128: two workgroups take half of the output's dimensions each and both compute the scores: half as much again in
 // products, but a row's registers are fewer.  Four prompts of 2k-3k tokens, 16 / 4 heads of 256: 959 us with the head in one
-// workgroup, 805 in two with one wave a SIMD, 535 with two (960, 740 where pages are of 16 tokens).
+// workgroup, 805 in two with one wave a SIMD, 535 with two (960, 740 where pages are of 16 tokens).  Two waves a SIMD leave 256 registers,
+// of which these variants spill 44 to 68 (f32 rows, one wave, 512 registers: 27 to 76); that is part of
+// those times.  So are the 6 to 16 that heads of 65 to 128 spill with a page number a lane.
 constexpr int value_parts(int padded_dim) { return padded_dim > 128 ? 2 : 1; }
 template <typename T, typename Code, int DP, bool EXACT, bool ONE, int WAVES>
 static __global__ __launch_bounds__(WAVES * kWave, DP <= 64 || RowType<T>::QP == 1 ? 2 : 1) void kvattention_tiles_kernel(const AttArgs a) {

@@ -493,7 +493,8 @@ typedef struct dxh_heads {
  *   of the first rotary.dim values the pairs (i, i + rotary.dim/2), or (2i, 2i + 1) with `interleaved`, are turned by the
  *   angle whose cosine and sine are cos[p][i] and sin[p][i], p = positions[row]:  y_a = n_a c - n_b s,  y_b = n_b c + n_a s;
  *   the other values of the head pass unchanged.
- * Computed in fp32, one rounding of the result.  cos / sin: fp32 [table_rows, rotary.dim / 2]; a position outside the table
+ * Computed in fp32, one rounding of the result: squares below 2^-149 are lost, and a head whose squares' sum is past the largest float
+ * comes out as zeros.  cos / sin: fp32 [table_rows, rotary.dim / 2]; a position outside the table
  * is clamped into it; positions NULL: 0, 1, 2 ...  rotary NULL or rotary.dim = 0: no rotation.  y may be x itself (the same
  * pointer and strides); any other overlap is not allowed, and DXH_ERR_ARG where a result begins in the place of another result, a
  * weight, a table or another part's input.  dtypes f32 f16 bf16, weights of the same dtype or f32, dim a
@@ -510,8 +511,8 @@ typedef struct dxh_normrope_part {
     dxh_heads x;
     dxh_heads y;          /* forward: the result; backward: the gradient that comes in */
     dxh_heads dx;         /* backward: the gradient of x (may be y itself); forward: not used */
-    const void *weight;   /* [dim], or NULL */
-    float *dweight;       /* backward: [dim] fp32, overwritten, or NULL; forward: not used */
+    const void *weight;   /* [dim], 16-byte aligned, else DXH_ERR_ALIGN; or NULL */
+    float *dweight;       /* backward: [dim] fp32, overwritten with norm = 1, left as it is with norm = 0 (there is no weight), or NULL; forward: not used */
     int32_t heads, norm;  /* norm: 1 on, 0 off */
     int32_t weight_dtype;
 } dxh_normrope_part;
@@ -543,8 +544,8 @@ DXH_API int dxh_normrope_backward(int dtype, const dxh_normrope_part *parts, int
  * has no place in the cache: it is not written and reads as zeros.  Rows of a sequence beyond max_rows and rows behind the
  * last sequence are left as they are; offsets outside [0, rows] are clamped into it: no content of the device arrays makes
  * a call touch memory outside its tensors.
- * Nothing of the device arrays is read on the host, so a recorded graph follows them as they change.  Rows, results and the cache
- * must not overlap; DXH_ERR_ARG where one begins in the place of another. */
+ * Nothing of the device arrays is read on the host, so a recorded graph follows them as they change.  Neither rows nor results may
+ * overlap the cache, its table or the arrays of a dxh_kvrows; DXH_ERR_ARG where one begins in the place of another. */
 typedef struct dxh_kvcache {
     void *k, *v;
     float *k_scale, *v_scale;

@@ -608,3 +608,19 @@ def test_what_eight_bits_cost(dxh, code):
                 bar = np.broadcast_to(dv[:, kh], V[:, kh].shape).max(0) + (np.exp(2 * e) - 1) * (p @ np.abs(V[:, kh])) + 1e-5
                 err = np.abs(out[r, h].double().cpu().numpy() - p @ V[:, kh])
                 assert (err <= bar).all(), (b, t, h, float((err / bar).max()))
+
+
+@pytest.mark.parametrize("name,code,page,dim", [("bf16", "i8", 16, 64), ("f32", "e4m3", 64, 128), ("f16", "i8", 128, 80), ("bf16", "e4m3", 32, 256)])
+def test_a_table_wider_than_its_sequences(dxh, name, code, page, dim):
+    """a table of a context limit over short sequences: the calls are planned as if they were long, and slices without tokens take no part"""
+    c = R.Cache(code, page, 1, dim, 3, -(-20000 // page), seed=32)
+    c.table[:, -(-800 // page):] = [[-1], [1 << 30], [-7]]
+    for counts, lengths in (((1, 1, 1), (777, 1, 0)), ((3, 8, 2), (700, 8, 65)), ((40, 1, 5), (90, 800, 5))):
+        rows = R.Rows(counts, lengths)
+        need = C.c_size_t(0)
+        dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.upload(), rows.upload(), R.DT[name], 3, C.byref(need)))
+        assert need.value >= 2 * rows.rows * 3 * (dim + 2) * 4
+        a = check(dxh, c, rows, name, 3)
+        assert torch.equal(a, check(dxh, c, rows, name, 3))
+        check(dxh, c, rows, name, 3, window=50)
+        check(dxh, c, many(counts, lengths), name, 3)

@@ -477,6 +477,14 @@ class PoolCache(R.Cache):
         return dx.KvCache(*[t.data_ptr() for t in self.dev], self.dev_table.data_ptr(), pages, self.per_seq, self.page, self.heads, self.dim, R.CODE[self.code])
 
 
+class WideCache(PoolCache):
+    """The same with a table so wide that its sequences could hold more codes than the last-level cache: they are read past it where pages are of 64 tokens."""
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.table, self.per_seq = np.pad(self.table, ((0, 0), (0, 1200)), constant_values=-1), self.per_seq + 1200
+
+
 @pytest.mark.parametrize("code,page,dim", [("i8", 64, 128), ("e4m3", 128, 64)])
 def test_the_pool_around_a_cache_changes_no_bit(dxh, code, page, dim):
     """what serves a call goes by what its rows can read: the pages of their sequences, not the pool that those are taken from"""
@@ -508,20 +516,19 @@ def workgroups(L, c, rows, name, q_heads):
     return len(rows.counts) * c.heads * -(-rows.max_rows * q_heads // c.heads // 16) * splits
 
 
-@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("code,page,dim", [("i8", 16, 64), ("e4m3", 16, 128), ("e4m3", 32, 80), ("i8", 32, 128), ("i8", 64, 128), ("e4m3", 64, 64), ("i8", 128, 80), ("e4m3", 128, 128), ("i8", 64, 256), ("e4m3", 16, 192)])
-def test_batches_that_fill_the_card(dxh, code, page, dim, name):
-    """more workgroups than CUs, with sequences whose waves walk several tiles each: missing pages, windows that begin inside a tile, the worst codes
-    and scales where no row sees them, a NaN among the values of a late token"""
+def ragged_batch(L, name, code, page, dim, hk, kind=R.Cache):
+    """40 sequences of up to 1500 tokens, whose waves walk several tiles each: missing pages, windows that begin inside a tile, the worst codes and scales
+    where no row sees them, a NaN among the values of a late token"""
+    hq = 2 * hk
     per = -(-1500 // page)
     lengths = [1 + 487 * i % 1500 for i in range(38)] + [1500, 1490]
     rows = R.Rows([1 + i % 2 for i in range(38)] + [2, 1], lengths, extra=1)
-    c = R.Cache(code, page, 4, dim, 40, per, seed=29, missing=[(0, 0, -1), (3, 0, 1 << 30), (38, 3, -1), (38, per - 2, -9), (39, 1, 1 << 30)])
-    assert workgroups(dxh, c, rows, name, 8) > 256
-    a = check(dxh, c, rows, name, 8)
-    assert torch.equal(a, check(dxh, c, rows, name, 8))
+    c = kind(code, page, hk, dim, 40, per, seed=29, missing=[(0, 0, -1), (3, 0, 1 << 30), (38, 3, -1), (38, per - 2, -9), (39, 1, 1 << 30)])
+    assert (workgroups(L, c, rows, name, hq) > 256) == (hk > 1 or kind is WideCache)
+    a = check(L, c, rows, name, hq)
+    assert torch.equal(a, check(L, c, rows, name, hq))
     for window, causal in ((1000, 1), (333, 0)):
-        check(dxh, c, rows, name, 8, window=window, causal=causal)
+        check(L, c, rows, name, hq, window=window, causal=causal)
     seen = np.zeros((c.pages, page), bool)
     for b, r, t in rows.each():
         for slot in range(-(-(t + 1) // page) if t >= 0 else 0):
@@ -531,19 +538,39 @@ def test_batches_that_fill_the_card(dxh, code, page, dim, name):
     c.v[~np.broadcast_to(seen[:, None, None, :], c.v.shape)] = 127
     c.ks[~seen.any(1)] = np.nan
     c.vs[~seen.any(1)] = np.inf
-    assert torch.equal(a, check(dxh, c, rows, name, 8))
+    assert torch.equal(a, check(L, c, rows, name, hq))
     if code == "e4m3":  # the last two tokens of the longest sequence: its first row sees one of them
         first = int(rows.offsets[38])
-        c.v[c.page_of(38, 1498 // page), 1, 5, 1498 % page] = -1
-        c.v[c.page_of(38, 1499 // page), 2, 6, 1499 % page] = 127
+        c.v[c.page_of(38, 1498 // page), 0, 5, 1498 % page] = -1
+        c.v[c.page_of(38, 1499 // page), hk - 1, 6, 1499 % page] = 127
         out = torch.full_like(a, 7.0)
-        q = torch.randn(rows.rows, 8, dim, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(R.TT[name])
-        call(dxh, c.upload(), rows.upload(), name, q, out, None, dim ** -0.5, 1, 0)
-        assert torch.isnan(out[first:first + 2, 2:4, 5]).all() and torch.isnan(out[first + 1, 4:6, 6]).all()
-        same = torch.ones(rows.rows, 8, dtype=torch.bool, device="cuda")
-        same[first:first + 2, 2:4] = False
-        same[first + 1, 4:6] = False
+        q = torch.randn(rows.rows, hq, dim, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(R.TT[name])
+        call(L, c.upload(), rows.upload(), name, q, out, None, dim ** -0.5, 1, 0)
+        assert torch.isnan(out[first:first + 2, :2, 5]).all() and torch.isnan(out[first + 1, hq - 2:, 6]).all()
+        same = torch.ones(rows.rows, hq, dtype=torch.bool, device="cuda")
+        same[first:first + 2, :2] = False
+        same[first + 1, hq - 2:] = False
         assert torch.equal(out[same], a[same])
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code,page,dim", [("i8", 16, 64), ("e4m3", 16, 128), ("e4m3", 32, 80), ("i8", 32, 128), ("i8", 64, 128), ("e4m3", 64, 64), ("i8", 128, 80), ("e4m3", 128, 128), ("i8", 64, 256), ("e4m3", 16, 192)])
+def test_batches_that_fill_the_card(dxh, code, page, dim, name):
+    ragged_batch(dxh, name, code, page, dim, 4)  # more workgroups than CUs
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("code,page,dim", [("e4m3", 16, 64), ("i8", 32, 80), ("e4m3", 64, 128), ("e4m3", 128, 96), ("e4m3", 32, 128)])
+def test_batches_that_leave_cus_idle(dxh, code, page, dim, name):
+    ragged_batch(dxh, name, code, page, dim, 1)  # eight waves a workgroup, two tiles a wave in its slice
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("code,dim,hk", [("e4m3", 64, 4), ("i8", 128, 4), ("e4m3", 128, 1), ("e4m3", 80, 2), ("i8", 256, 2), ("e4m3", 192, 1)])
+def test_batches_read_past_the_last_level_cache(dxh, code, dim, hk, name):
+    c = WideCache(code, 64, hk, dim, 40, 24, seed=1)
+    assert min(c.pool // (hk * 64 * dim), 40 * c.per_seq) * hk * 64 * dim * 2 > 340 << 20
+    ragged_batch(dxh, name, code, 64, dim, hk, WideCache)
 
 
 @pytest.mark.parametrize("name", ["f16", "bf16"])

@@ -5,7 +5,8 @@
 //   1. top = max |x| over the new rows of the page, 16-byte loads along a row, compared as the whole numbers that their bits
 //      are (two at a time for 16-bit rows): an infinity or a NaN then shows as a top past the largest finite number, and only
 //      such a page pays for clamps and NaN checks;
-//   2. scale = max(top / max code, 2^-100), at least the old scale if older tokens of the sequence are in the page;
+//   2. scale = max(top / max code, 2^-100), at least the old scale if older tokens of the sequence are in the page (an old scale that
+//      is no finite number stays);
 //   3. codes.  Keys: a lane makes 16 codes of one token.  Values lie with the tokens innermost: a lane makes 16 tokens of one
 //      dimension, lanes along the dimensions, so that each of its 16 reads is one row of LDS (or one line of memory) for the
 //      wave.  Older codes are only read when the scale grew, or where they share a 16-token piece with new ones.
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(THREADS) void kvcache_write_kernel(const RowsArgs a
     uint8_t *codes = (which ? a.kv.v : a.kv.k) + where * P * D;
     const float old = t0 > 0 ? *scale_at : 0.f;
     float scale = __builtin_fmaxf(top * Code::inv_max, 0x1p-100f);
-    if (t0 > 0) scale = __builtin_fmaxf(scale, old);
+    if (t0 > 0) scale = old - old == 0.f ? __builtin_fmaxf(scale, old) : old;  // the older tokens have no values: the page shows it
     const bool grew = t0 > 0 && scale > old;
     const float inv = 1.f / scale, again = old * inv;
     if (THREADS > kWave && t0 > 0) __syncthreads();  // every wave has the old scale

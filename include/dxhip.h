@@ -563,7 +563,8 @@ typedef struct dxh_kvrows {
 /* Quantises new keys and values into the cache.  For every page and head that rows fall into, in fp32 with one rounding a step:
  *   top   = the largest |x| among them (NaN ignored, infinities as FLT_MAX)
  *   scale = max(top * c, 2^-100), c = the fp32 value nearest to 1/127 (int8) or 1/448 (e4m3); if the page holds older tokens
- *           of the sequence (before the first row) at least its old scale
+ *           of the sequence (before the first row) at least its old scale (one that is not finite stays, and the page's new codes
+ *           mean nothing)
  *   code  = x * (1 / scale), clamped to +-127 or +-448, rounded to nearest even (a NaN becomes 0 in int8, NaN in e4m3)
  * and, if older tokens are there and the scale grew, their codes become code * (old scale * (1 / scale)) rounded the same way.
  * Codes of a page behind the last row are left as they are.  The pages that two sequences write must differ (a page shared

@@ -169,3 +169,29 @@ def test_large_cache(dxh):
             assert torch.allclose(scales[place], top.clamp(min=least), rtol=1e-6)
             off = ((b - x)[rows_of_page].abs().amax((0, 2)) / scales[place]).max().item()
             assert off <= 0.501, (place, off)
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("page,dim", [(16, 32), (64, 128)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_broken_scale_is_not_written_over(dxh, bad, page, dim, code):
+    """older tokens whose page has a scale that is no finite number have no values: a new token in their page does not make them look as if they had, and the
+    attention goes on giving NaN; a page that begins with the new rows gets a scale of its own"""
+    c = R.Cache(code, page, 2, dim, 3, 2, seed=8)
+    c.ks[c.page_of(0, 0), 1] = c.vs[c.page_of(1, 0), 0] = c.ks[c.page_of(2, 0), 0] = bad
+    c.desc = c.upload()
+    rows = R.Rows((1, 2, page), (page // 2, page - 1, page))  # the third sequence's page is new
+    desc = rows.upload()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    k, v = (torch.randn(rows.rows, 2, dim, generator=g, device="cuda") * 100 for _ in range(2))
+    dx.check(dxh.dxh_kvcache_write(c.desc, desc, dx.F32, R.heads(k), R.heads(v), stream()))
+    _, _, ks, vs = c.download()
+    same = lambda x: x == bad or (np.isnan(bad) and np.isnan(x))  # noqa: E731
+    assert same(ks[c.page_of(0, 0), 1]) and same(vs[c.page_of(1, 0), 0])
+    assert np.isfinite(ks[c.page_of(0, 0), 0]) and np.isfinite(vs[c.page_of(0, 0)]).all() and np.isfinite(ks[c.page_of(2, 0)]).all() and np.isfinite(vs[c.page_of(2, 0)]).all()
+    q, out, ws, need = torch.randn(rows.rows, 2, dim, generator=g, device="cuda"), torch.empty(rows.rows, 2, dim, device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda"), C.c_size_t(0)
+    dx.check(dxh.dxh_kvcache_attention_workspace_bytes(c.desc, desc, dx.F32, 2, C.byref(need)))
+    assert need.value <= ws.numel()
+    dx.check(dxh.dxh_kvcache_attention(c.desc, desc, dx.F32, 2, R.heads(q), R.heads(out), None, 0.1, 1, 0, ws.data_ptr(), ws.numel(), stream()))
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(out[1:3, 0]).all()
+    assert torch.isfinite(out[0, 0]).all() and torch.isfinite(out[1:3, 1]).all() and torch.isfinite(out[3:]).all()
